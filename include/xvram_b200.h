@@ -129,7 +129,8 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_sgemm_device_noalloc(
 
 /* Synchronises `stream`, then returns and clears the device's sticky kernel error word
  * (nonzero: a pipeline wait inside a kernel ran out of time and the kernel returned
- * without finishing).  No reference counterpart (the reference has no kernels). */
+ * without finishing; the bytes from the lowest: FFMA, three-term TF32, gated, MXFP4 kernels).
+ * No reference counterpart (the reference has no kernels). */
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_kernel_status(uint64_t stream,
                                                                 uint32_t* word);
 
@@ -370,6 +371,102 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_bias_activation(uint64_t y, in
                                                                  uint64_t bias,
                                                                  uint32_t activation,
                                                                  uint64_t stream);
+
+/* Activations of the gated blocks below: v sigmoid(v), v Phi(v) (the exact GELU), the GELU's
+ * tanh form, max(v, 0) and sigmoid(v). */
+enum {
+  XVRAM_B200_GATE_SILU = 0,
+  XVRAM_B200_GATE_GELU = 1,
+  XVRAM_B200_GATE_GELU_TANH = 2,
+  XVRAM_B200_GATE_RELU = 3,
+  XVRAM_B200_GATE_SIGMOID = 4
+};
+
+/*
+ * The gated feed-forward block over device memory:
+ *   out = act(x Wg^T + bg) * (x Wu^T + bu)        x: m x k, Wg and Wu: h x k, out: m x h
+ * FP16 and BF16 run both projections, the biases, the activation and the product in one
+ * tensor-core kernel (FP32 accumulation, one rounding); FP32 is strict FP32 (FFMA).  No
+ * reference counterpart (its torch route offers bias-free mm / linear alone).
+ *
+ * Storage: a row's k values contiguous, leading dimensions in elements between rows (the
+ * column-major k x rows matrix); x_transposed / w_transposed = 1 for operands stored the
+ * other way (k rows of m or h values).  FP16 / BF16 operands need 16-byte aligned bases and
+ * leading dimensions that are multiples of 8; FP32 operands any.  Biases (0 for none) hold h
+ * values of the data type.  pre_gate and pre_up, both or neither, receive x Wg^T + bg and
+ * x Wu^T + bu in FP32 (m x h, ld_pre a multiple of 4, 16-byte aligned) for the backward pass.
+ * The workspace (256-byte aligned, xvram_b200_gated_workspace_bytes) may be reused once the
+ * call's work on `stream` is done.
+ */
+typedef struct xvram_b200_gated_v1 {
+  uint32_t struct_size; /* sizeof(xvram_b200_gated_v1) */
+  uint32_t data_type;   /* XVRAM_DATA_FP16, _BF16 or _FP32 */
+  uint32_t activation;  /* XVRAM_B200_GATE_* */
+  uint32_t x_transposed, w_transposed;
+  uint32_t reserved0;
+  int64_t m, h, k; /* m and h >= 0, k >= 1 */
+  uint64_t x, w_gate, w_up;
+  int64_t ldx, ld_gate, ld_up;
+  uint64_t bias_gate, bias_up;
+  uint64_t pre_gate, pre_up;
+  int64_t ld_pre;
+  uint64_t workspace, workspace_bytes;
+  uint64_t stream;
+} xvram_b200_gated_v1;
+
+/* Bytes of workspace the forward (backward = 0) or backward pass of this problem needs; only
+ * the type, the sizes, the transpositions and whether pre_gate is set are read.  0 for an
+ * invalid problem. */
+XVRAM_B200_API uint64_t XVRAM_CALL
+xvram_b200_gated_workspace_bytes(const xvram_b200_gated_v1* problem, uint32_t backward);
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_forward(const xvram_b200_gated_v1* problem,
+                                                              uint64_t out, int64_t ld_out);
+
+/* Gradients of the block from dout (m x h) and the forward's pre_gate and pre_up, which must be
+ * set; each of dx (m x k), dw_gate and dw_up (h x k, ld_dw), db_gate and db_up (h) may be 0 when
+ * it is not wanted.  Gradients have the data type and are stored with contiguous rows whatever
+ * the operands' transposition.  For FP16 / BF16 the gradients of the pre-activations are rounded
+ * to the data type once, as the tensor cores' operands; all sums are FP32.  Results do not depend
+ * on timing.  With m = 0 the weights' and biases' gradients are zeros. */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_backward(
+    const xvram_b200_gated_v1* problem, uint64_t dout, int64_t ld_dout, uint64_t dx, int64_t ld_dx,
+    uint64_t dw_gate, uint64_t dw_up, int64_t ld_dw, uint64_t db_gate, uint64_t db_up);
+
+/*
+ * MXFP4 matrices: blocks of 32 neighbouring values of a row share a scale 2^(s - 127) (one
+ * byte s, E8M0), s = clamp(floor(log2 max|v|) - 2, -127, 127) + 127; the elements are E2M1
+ * (0, .5, 1, 1.5, 2, 3, 4, 6), v / scale rounded to nearest even and saturating at 6.  A block
+ * with a NaN or an infinity has the scale byte 255 and reads back as NaN.
+ *   codes:  rows x ceil(cols / 32) x 16 bytes, the even element in the low half of a byte;
+ *   scales: tiles of 128 rows x 4 blocks, 512 bytes each, [ceil(rows / 128)][ceil(cols / 128)];
+ *           row r, block b of a tile at byte (r % 32) * 16 + (r / 32) * 4 + b.
+ * Codes past the last column must be 0 and scales past the last row or block any value but 255
+ * (the quantisation writes 0 and 127).  Both 16-byte aligned.  No reference counterpart.
+ */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_bytes(int64_t rows, int64_t cols,
+                                                            uint64_t* code_bytes,
+                                                            uint64_t* scale_bytes);
+/* src: rows of `cols` contiguous values, lds elements apart (FP16, BF16 or FP32). */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_quantize(
+    uint32_t data_type, int64_t rows, int64_t cols, uint64_t src, int64_t lds, uint64_t codes,
+    uint64_t scales, uint64_t stream);
+/* The values that codes and scales stand for, rounded to the data type (exact in FP32). */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
+    uint32_t data_type, int64_t rows, int64_t cols, uint64_t codes, uint64_t scales, uint64_t dst,
+    int64_t ldd, uint64_t stream);
+/* out (m x n) = x W^T (+ bias) (then ReLU): x m x k and W n x k, both MXFP4, on the block-scaled
+ * tensor-core MMA with FP32 accumulation; out and bias (n values, or 0) of out_type. */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_linear(
+    uint32_t out_type, int64_t m, int64_t n, int64_t k, uint64_t x_codes, uint64_t x_scales,
+    uint64_t w_codes, uint64_t w_scales, uint64_t bias, uint32_t activation, uint64_t out,
+    int64_t ld_out, uint64_t stream);
+/* The gated block over MXFP4 operands: out (m x h) = act(x Wg^T + bg) * (x Wu^T + bu). */
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_gated(
+    uint32_t out_type, uint32_t activation, int64_t m, int64_t h, int64_t k, uint64_t x_codes,
+    uint64_t x_scales, uint64_t gate_codes, uint64_t gate_scales, uint64_t up_codes,
+    uint64_t up_scales, uint64_t bias_gate, uint64_t bias_up, uint64_t out, int64_t ld_out,
+    uint64_t stream);
 
 /* Extra state of the compat adapter's runtime (not in the reference telemetry). */
 typedef struct xvram_b200_runtime_info_v1 {

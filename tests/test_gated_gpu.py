@@ -1,0 +1,73 @@
+"""The gated feed-forward block (xvram_b200.torch_bridge.gated_linear) and its gradients
+against 64-bit references, with the bounds that feed_util derives."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():  # pragma: no cover
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+import feed_util as fu  # noqa: E402
+from xvram_b200 import device as xd  # noqa: E402
+from xvram_b200 import torch_bridge as tb  # noqa: E402
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+# (batch, out, in): one element, fewer than a tile, whole tiles, one past them, long sums.
+SHAPES = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (128, 128, 64), (129, 257, 65), (5, 300, 1000),
+          (257, 136, 520)]
+
+
+def problem(kind, m, h, k, seed=0, bias=True):
+    x = fu.normal((m, k), kind, seed)
+    wg, wu = (fu.normal((h, k), kind, seed + i, k ** -0.5) for i in (1, 2))
+    bg, bu = (fu.normal((h,), kind, seed + i, 0.5) if bias else None for i in (3, 4))
+    return x, wg, wu, bg, bu
+
+
+def check_forward(args, act):
+    ref = fu.Gated(*args, act, args[0].dtype)
+    got = tb.gated_linear(*args, activation=act)
+    assert got.dtype == args[0].dtype and got.is_contiguous()
+    fu.within(got, ref.h, ref.h_tol, "h")
+    assert xd.kernel_status() == 0
+    return got
+
+
+def check_gradients(args, act, dh):
+    ref = fu.Gated(*args, act, args[0].dtype)
+    leaves = [None if t is None else t.detach().requires_grad_() for t in args]
+    h = tb.gated_linear(*leaves, activation=act)
+    fu.within(h.detach(), ref.h, ref.h_tol, "h")
+    h.backward(dh)
+    want = ref.backward(dh)
+    for n, t in zip(("dx", "dw_gate", "dw_up", "db_gate", "db_up"), leaves):
+        if t is not None:
+            fu.within(t.grad, *want[n], n)
+    assert xd.kernel_status() == 0
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("kind", TYPES)
+def test_forward(kind, shape):
+    check_forward(problem(kind, *shape), "silu")
+
+
+@pytest.mark.parametrize("act", fu.ACTS)
+@pytest.mark.parametrize("kind", TYPES)
+def test_forward_activations_without_bias(kind, act):
+    check_forward(problem(kind, 33, 72, 96, 5, bias=False), act)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("kind", TYPES)
+def test_gradients(kind, shape):
+    m, h, k = shape
+    check_gradients(problem(kind, m, h, k, 10), "silu", fu.normal((m, h), kind, 20))
+
+
+@pytest.mark.parametrize("act", fu.ACTS)
+@pytest.mark.parametrize("kind", TYPES)
+def test_gradients_of_each_activation(kind, act):
+    check_gradients(problem(kind, 70, 144, 40, 30), act, fu.normal((70, 144), kind, 31))

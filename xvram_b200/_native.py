@@ -86,6 +86,18 @@ class ShardPlan(C.Structure):
                 ("gathers", u64), ("h2d_bytes", u64), ("d2h_bytes", u64)]
 
 
+class Gated(C.Structure):
+    """xvram_b200_gated_v1 (include/xvram_b200.h)."""
+
+    _fields_ = [("struct_size", u32), ("data_type", u32), ("activation", u32),
+                ("x_transposed", u32), ("w_transposed", u32), ("reserved0", u32),
+                ("m", i64), ("h", i64), ("k", i64),
+                ("x", u64), ("w_gate", u64), ("w_up", u64),
+                ("ldx", i64), ("ld_gate", i64), ("ld_up", i64),
+                ("bias_gate", u64), ("bias_up", u64), ("pre_gate", u64), ("pre_up", u64),
+                ("ld_pre", i64), ("workspace", u64), ("workspace_bytes", u64), ("stream", u64)]
+
+
 def _load() -> C.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -158,6 +170,25 @@ def _load() -> C.CDLL:
     lib.xvram_get_api.restype = u32
     lib.xvram_b200_bias_activation.argtypes = [u64, i64, i64, i64, u64, u32, u64]
     lib.xvram_b200_bias_activation.restype = u32
+    gated = C.POINTER(Gated)
+    lib.xvram_b200_gated_workspace_bytes.argtypes = [gated, u32]
+    lib.xvram_b200_gated_workspace_bytes.restype = u64
+    lib.xvram_b200_gated_forward.argtypes = [gated, u64, i64]
+    lib.xvram_b200_gated_forward.restype = u32
+    lib.xvram_b200_gated_backward.argtypes = [gated, u64, i64, u64, i64, u64, u64, i64, u64, u64]
+    lib.xvram_b200_gated_backward.restype = u32
+    lib.xvram_b200_mxfp4_bytes.argtypes = [i64, i64, C.POINTER(u64), C.POINTER(u64)]
+    lib.xvram_b200_mxfp4_bytes.restype = u32
+    lib.xvram_b200_mxfp4_quantize.argtypes = [u32, i64, i64, u64, i64, u64, u64, u64]
+    lib.xvram_b200_mxfp4_quantize.restype = u32
+    lib.xvram_b200_mxfp4_dequantize.argtypes = [u32, i64, i64, u64, u64, u64, i64, u64]
+    lib.xvram_b200_mxfp4_dequantize.restype = u32
+    lib.xvram_b200_mxfp4_linear.argtypes = [u32, i64, i64, i64, u64, u64, u64, u64, u64, u32, u64,
+                                            i64, u64]
+    lib.xvram_b200_mxfp4_linear.restype = u32
+    lib.xvram_b200_mxfp4_gated.argtypes = [u32, u32, i64, i64, i64, u64, u64, u64, u64, u64, u64,
+                                           u64, u64, u64, i64, u64]
+    lib.xvram_b200_mxfp4_gated.restype = u32
     lib.xvram_b200_digest_bench.argtypes = [vp, u64, u64, C.POINTER(u64)]
     lib.xvram_b200_digest_bench.restype = None
     lib.xvram_b200_digest_compat.argtypes = [vp, u64, C.POINTER(u64)]
@@ -210,6 +241,14 @@ EXPORTED = (
     "xvram_b200_validate_gemm_typed",
     "xvram_b200_gemm_typed_workspace_bytes",
     "xvram_b200_gemm_device_typed",
+    "xvram_b200_gated_workspace_bytes",
+    "xvram_b200_gated_forward",
+    "xvram_b200_gated_backward",
+    "xvram_b200_mxfp4_bytes",
+    "xvram_b200_mxfp4_quantize",
+    "xvram_b200_mxfp4_dequantize",
+    "xvram_b200_mxfp4_linear",
+    "xvram_b200_mxfp4_gated",
     "xvram_b200_ffma_probe",
     "xvram_b200_ffma2_probe",
     "xvram_b200_compat_runtime_info",

@@ -102,6 +102,66 @@ cudaError_t gemm_typed(uint32_t ab_type, uint32_t c_type, int compute, int op_a,
 cudaError_t convert_matrix(uint32_t src_type, const void* src, long long lds, uint32_t dst_type,
                            void* dst, long long ldd, int rows, int cols, cudaStream_t stream);
 
+// The gated feed-forward block (gated.cu).  x holds m rows of k inputs, the weights h rows of k
+// (transposed: stored k x rows instead); leading dimensions in elements.  16-bit operands need
+// 16-byte aligned bases and leading dimensions that are multiples of 8 (cudaErrorInvalidValue
+// otherwise); pre_gate and pre_up (both or neither; FP32, 16-byte aligned, ld_pre a multiple
+// of 4) receive the pre-activations, biases included.  m, h and k are positive.
+enum class GatedType { f16 = 0, bf16 = 1, f32 = 2 };
+struct GatedProblem {
+  GatedType type = GatedType::f32;
+  int act = 0;
+  int m = 0, h = 0, k = 0;
+  bool x_transposed = false, w_transposed = false;
+  const void *x = nullptr, *w_gate = nullptr, *w_up = nullptr;
+  long long ldx = 0, ld_gate = 0, ld_up = 0;
+  const void *bias_gate = nullptr, *bias_up = nullptr;
+  float *pre_gate = nullptr, *pre_up = nullptr;
+  long long ld_pre = 0;
+};
+// Gradients to compute (null: not wanted), from dh (m x h).
+struct GatedGradients {
+  const void* dh = nullptr;
+  long long lddh = 0;
+  void* dx = nullptr;
+  long long lddx = 0;
+  void *dw_gate = nullptr, *dw_up = nullptr;
+  long long ld_dw = 0;
+  void *db_gate = nullptr, *db_up = nullptr;
+};
+uint64_t gated_partial_bytes(int m, int h);
+uint64_t gated_workspace_bytes(const GatedProblem& q, bool backward);
+cudaError_t gated_forward(const GatedProblem& q, void* out, long long ldo, void* workspace,
+                          uint64_t workspace_bytes, cudaStream_t stream);
+cudaError_t gated_backward(const GatedProblem& q, const GatedGradients& d, void* workspace,
+                           uint64_t workspace_bytes, cudaStream_t stream);
+cudaError_t read_and_clear_kernel_error_gated(unsigned int* out, cudaStream_t stream);
+
+// MXFP4 (mxfp4.cu): codes rows x ceil(cols / 32) x 16 bytes, scales ceil(rows / 128) x
+// ceil(cols / 128) tiles of 512 bytes, both 16-byte aligned.  Sizes are positive; lds and ldd in
+// elements of `type`.
+struct Mxfp4Operand {
+  const unsigned char *codes = nullptr, *scales = nullptr;
+};
+// out = a b[0]^T (+ bias[0], ReLU), or with b[1] act(a b[0]^T + bias[0]) * (a b[1]^T + bias[1]);
+// out and the biases are of `type`.
+struct Mxfp4Product {
+  GatedType type = GatedType::f32;
+  int m = 0, n = 0, k = 0, act = 0;
+  bool relu = false;
+  Mxfp4Operand a, b[2];
+  const void* bias[2] = {nullptr, nullptr};
+  void* out = nullptr;
+  long long ldo = 0;
+};
+cudaError_t mxfp4_quantize(GatedType type, const void* src, long long lds, int rows, int cols,
+                           unsigned char* codes, unsigned char* scales, cudaStream_t stream);
+cudaError_t mxfp4_dequantize(GatedType type, const unsigned char* codes,
+                             const unsigned char* scales, int rows, int cols, void* dst,
+                             long long ldd, cudaStream_t stream);
+cudaError_t mxfp4_product(const Mxfp4Product& q, cudaStream_t stream);
+cudaError_t read_and_clear_kernel_error_mxfp4(unsigned int* out, cudaStream_t stream);
+
 // Reads (synchronising `stream`) and clears the device's sticky kernel error word.
 cudaError_t read_and_clear_kernel_error(unsigned int* out, cudaStream_t stream);
 cudaError_t read_and_clear_kernel_error_tc(unsigned int* out, cudaStream_t stream);

@@ -107,6 +107,60 @@ PlanStatus plan_for(uint32_t op_a, uint32_t op_b, int64_t m, int64_t n, int64_t 
   return make_panel_plan(p, lim, plan);
 }
 
+void* pointer(uint64_t p) { return reinterpret_cast<void*>(p); }
+unsigned char* bytes(uint64_t p) { return reinterpret_cast<unsigned char*>(p); }
+
+bool element_aligned(uint64_t p, uint32_t data_type) {
+  return p % (data_type == XVRAM_DATA_FP32 ? 4 : 2) == 0;
+}
+
+// The checked problem; false when an argument is invalid.  `operands` also checks the pointers
+// and leading dimensions (the workspace query has none).
+bool gated_problem(const xvram_b200_gated_v1& d, bool operands, GatedProblem* q) {
+  if (d.struct_size < sizeof(d) || d.data_type > XVRAM_DATA_FP32 ||
+      d.activation > XVRAM_B200_GATE_SIGMOID || d.x_transposed > 1 || d.w_transposed > 1 ||
+      d.m < 0 || d.h < 0 || d.k < 1 || d.m > INT32_MAX || d.h > INT32_MAX || d.k > INT32_MAX)
+    return false;
+  if (operands && d.m > 0 && d.h > 0) {
+    const int64_t wx = d.x_transposed ? d.m : d.k, ww = d.w_transposed ? d.h : d.k;
+    if (!d.x || !d.w_gate || !d.w_up || d.ldx < wx || d.ld_gate < ww || d.ld_up < ww ||
+        !d.pre_gate != !d.pre_up)
+      return false;
+    if (d.pre_gate && (d.ld_pre < d.h || d.ld_pre % 4 || d.pre_gate % 16 || d.pre_up % 16))
+      return false;
+    for (uint64_t p : {d.x, d.w_gate, d.w_up, d.bias_gate, d.bias_up})
+      if (!element_aligned(p, d.data_type))
+        return false;
+  }
+  q->type = static_cast<GatedType>(d.data_type);
+  q->act = static_cast<int>(d.activation);
+  q->m = static_cast<int>(d.m);
+  q->h = static_cast<int>(d.h);
+  q->k = static_cast<int>(d.k);
+  q->x_transposed = d.x_transposed != 0;
+  q->w_transposed = d.w_transposed != 0;
+  q->x = pointer(d.x);
+  q->w_gate = pointer(d.w_gate);
+  q->w_up = pointer(d.w_up);
+  q->ldx = d.ldx;
+  q->ld_gate = d.ld_gate;
+  q->ld_up = d.ld_up;
+  q->bias_gate = pointer(d.bias_gate);
+  q->bias_up = pointer(d.bias_up);
+  q->pre_gate = static_cast<float*>(pointer(d.pre_gate));
+  q->pre_up = static_cast<float*>(pointer(d.pre_up));
+  q->ld_pre = d.ld_pre;
+  return true;
+}
+
+// Columns are at most 2^31 - 32, so that a padded row's length is an int.
+bool mxfp4_size(int64_t rows, int64_t cols) {
+  return rows >= 0 && cols >= 0 && rows <= INT32_MAX - 127 && cols <= INT32_MAX - 255;
+}
+bool mxfp4_operand(uint64_t codes, uint64_t scales) {
+  return codes && scales && codes % 16 == 0 && scales % 16 == 0;
+}
+
 } // namespace
 
 extern "C" {
@@ -202,11 +256,15 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_sgemm_device_ws(
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_kernel_status(uint64_t stream, uint32_t* word) {
   if (!word)
     return XVRAM_STATUS_INVALID_ARGUMENT;
-  unsigned int w = 0, wt = 0;
+  unsigned int w = 0, wt = 0, wg = 0, wm = 0;
   cudaError_t e = read_and_clear_kernel_error(&w, as_stream(stream));
   if (e == cudaSuccess)
     e = read_and_clear_kernel_error_tc(&wt, as_stream(stream));
-  *word = w | (wt << 8); // tensor-core kernel bits in the second byte
+  if (e == cudaSuccess)
+    e = read_and_clear_kernel_error_gated(&wg, as_stream(stream));
+  if (e == cudaSuccess)
+    e = read_and_clear_kernel_error_mxfp4(&wm, as_stream(stream));
+  *word = w | (wt << 8) | (wg << 16) | (wm << 24); // a byte per kernel family
   return from_cuda(e);
 }
 
@@ -420,6 +478,166 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_ffma2_probe(int32_t blocks, in
 XVRAM_B200_API xvram_status XVRAM_CALL
 xvram_b200_compat_runtime_info(xvram_b200_runtime_info_v1* out) {
   return compat_runtime_info(out);
+}
+
+XVRAM_B200_API uint64_t XVRAM_CALL
+xvram_b200_gated_workspace_bytes(const xvram_b200_gated_v1* problem, uint32_t backward) {
+  GatedProblem q;
+  if (!problem || problem->m == 0 || problem->h == 0 || !gated_problem(*problem, false, &q))
+    return 0;
+  return gated_workspace_bytes(q, backward != 0);
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_forward(const xvram_b200_gated_v1* problem,
+                                                              uint64_t out, int64_t ld_out) {
+  GatedProblem q;
+  if (!problem || !gated_problem(*problem, true, &q))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (q.m == 0 || q.h == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!out || ld_out < q.h || !element_aligned(out, problem->data_type))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  return from_cuda(gated_forward(q, pointer(out), ld_out, pointer(problem->workspace),
+                                 problem->workspace_bytes, as_stream(problem->stream)));
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_backward(
+    const xvram_b200_gated_v1* problem, uint64_t dout, int64_t ld_dout, uint64_t dx, int64_t ld_dx,
+    uint64_t dw_gate, uint64_t dw_up, int64_t ld_dw, uint64_t db_gate, uint64_t db_up) {
+  GatedProblem q;
+  if (!problem || !gated_problem(*problem, true, &q))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if ((dx && ld_dx < q.k) || ((dw_gate || dw_up) && ld_dw < q.k))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  for (uint64_t p : {dout, dx, dw_gate, dw_up, db_gate, db_up})
+    if (!element_aligned(p, problem->data_type))
+      return XVRAM_STATUS_INVALID_ARGUMENT;
+  cudaStream_t s = as_stream(problem->stream);
+  const uint64_t size = q.type == GatedType::f32 ? 4 : 2;
+  if (q.m == 0 || q.h == 0) { // empty sums
+    if (q.h == 0)
+      return dx && q.m ? from_cuda(cudaMemset2DAsync(pointer(dx), ld_dx * size, 0, q.k * size, q.m,
+                                                     s))
+                       : XVRAM_STATUS_SUCCESS;
+    for (uint64_t w : {dw_gate, dw_up})
+      if (w)
+        if (cudaError_t e = cudaMemset2DAsync(pointer(w), ld_dw * size, 0, q.k * size, q.h, s);
+            e != cudaSuccess)
+          return from_cuda(e);
+    for (uint64_t b : {db_gate, db_up})
+      if (b)
+        if (cudaError_t e = cudaMemsetAsync(pointer(b), 0, q.h * size, s); e != cudaSuccess)
+          return from_cuda(e);
+    return XVRAM_STATUS_SUCCESS;
+  }
+  if (!q.pre_gate || !dout || ld_dout < q.h)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  GatedGradients d;
+  d.dh = pointer(dout);
+  d.lddh = ld_dout;
+  d.dx = pointer(dx);
+  d.lddx = ld_dx;
+  d.dw_gate = pointer(dw_gate);
+  d.dw_up = pointer(dw_up);
+  d.ld_dw = ld_dw;
+  d.db_gate = pointer(db_gate);
+  d.db_up = pointer(db_up);
+  return from_cuda(gated_backward(q, d, pointer(problem->workspace), problem->workspace_bytes, s));
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_bytes(int64_t rows, int64_t cols,
+                                                            uint64_t* code_bytes,
+                                                            uint64_t* scale_bytes) {
+  if (!mxfp4_size(rows, cols) || !code_bytes || !scale_bytes)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  *code_bytes = static_cast<uint64_t>(rows) * ((cols + 31) / 32) * 16;
+  *scale_bytes = static_cast<uint64_t>((rows + 127) / 128) * ((cols + 127) / 128) * 512;
+  return XVRAM_STATUS_SUCCESS;
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_quantize(
+    uint32_t data_type, int64_t rows, int64_t cols, uint64_t src, int64_t lds, uint64_t codes,
+    uint64_t scales, uint64_t stream) {
+  if (data_type > XVRAM_DATA_FP32 || !mxfp4_size(rows, cols))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (rows == 0 || cols == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!src || lds < cols || !element_aligned(src, data_type) || !mxfp4_operand(codes, scales))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  return from_cuda(mxfp4_quantize(static_cast<GatedType>(data_type), pointer(src), lds,
+                                  static_cast<int>(rows), static_cast<int>(cols), bytes(codes),
+                                  bytes(scales), as_stream(stream)));
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
+    uint32_t data_type, int64_t rows, int64_t cols, uint64_t codes, uint64_t scales, uint64_t dst,
+    int64_t ldd, uint64_t stream) {
+  if (data_type > XVRAM_DATA_FP32 || !mxfp4_size(rows, cols))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (rows == 0 || cols == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!dst || ldd < cols || !element_aligned(dst, data_type) || !mxfp4_operand(codes, scales))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  return from_cuda(mxfp4_dequantize(static_cast<GatedType>(data_type), bytes(codes), bytes(scales),
+                                    static_cast<int>(rows), static_cast<int>(cols), pointer(dst),
+                                    ldd, as_stream(stream)));
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_linear(
+    uint32_t out_type, int64_t m, int64_t n, int64_t k, uint64_t x_codes, uint64_t x_scales,
+    uint64_t w_codes, uint64_t w_scales, uint64_t bias, uint32_t activation, uint64_t out,
+    int64_t ld_out, uint64_t stream) {
+  if (out_type > XVRAM_DATA_FP32 || activation > XVRAM_B200_ACTIVATION_RELU || !mxfp4_size(m, k) ||
+      !mxfp4_size(n, k) || k < 1)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (m == 0 || n == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!mxfp4_operand(x_codes, x_scales) || !mxfp4_operand(w_codes, w_scales) || !out ||
+      ld_out < n || !element_aligned(out, out_type) || !element_aligned(bias, out_type))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  Mxfp4Product q;
+  q.type = static_cast<GatedType>(out_type);
+  q.m = static_cast<int>(m);
+  q.n = static_cast<int>(n);
+  q.k = static_cast<int>(k);
+  q.relu = activation == XVRAM_B200_ACTIVATION_RELU;
+  q.a = {bytes(x_codes), bytes(x_scales)};
+  q.b[0] = {bytes(w_codes), bytes(w_scales)};
+  q.bias[0] = pointer(bias);
+  q.out = pointer(out);
+  q.ldo = ld_out;
+  return from_cuda(mxfp4_product(q, as_stream(stream)));
+}
+
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_gated(
+    uint32_t out_type, uint32_t activation, int64_t m, int64_t h, int64_t k, uint64_t x_codes,
+    uint64_t x_scales, uint64_t gate_codes, uint64_t gate_scales, uint64_t up_codes,
+    uint64_t up_scales, uint64_t bias_gate, uint64_t bias_up, uint64_t out, int64_t ld_out,
+    uint64_t stream) {
+  if (out_type > XVRAM_DATA_FP32 || activation > XVRAM_B200_GATE_SIGMOID || !mxfp4_size(m, k) ||
+      !mxfp4_size(h, k) || k < 1)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (m == 0 || h == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!mxfp4_operand(x_codes, x_scales) || !mxfp4_operand(gate_codes, gate_scales) ||
+      !mxfp4_operand(up_codes, up_scales) || !out || ld_out < h ||
+      !element_aligned(out, out_type) || !element_aligned(bias_gate, out_type) ||
+      !element_aligned(bias_up, out_type))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  Mxfp4Product q;
+  q.type = static_cast<GatedType>(out_type);
+  q.m = static_cast<int>(m);
+  q.n = static_cast<int>(h);
+  q.k = static_cast<int>(k);
+  q.act = static_cast<int>(activation);
+  q.a = {bytes(x_codes), bytes(x_scales)};
+  q.b[0] = {bytes(gate_codes), bytes(gate_scales)};
+  q.b[1] = {bytes(up_codes), bytes(up_scales)};
+  q.bias[0] = pointer(bias_gate);
+  q.bias[1] = pointer(bias_up);
+  q.out = pointer(out);
+  q.ldo = ld_out;
+  return from_cuda(mxfp4_product(q, as_stream(stream)));
 }
 
 } // extern "C"

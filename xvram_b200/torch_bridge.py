@@ -23,6 +23,14 @@ rounded to the type once), FP64 in FP64.  `tensor_cores=True` selects the three-
 kernel for float32 (FP32-accurate within max|err| / (K max|a| max|b|) <= 1e-6); the
 default is strict FP32 FFMA.  Bias and ReLU are float32 only (the reference route takes
 neither).  There is no CPU fallback: without a GPU every call raises.
+
+Beside `linear` stand the feed-forward operators (the reference has none of them), for CUDA
+tensors:
+
+* `gated_linear`, the gated block act(x Wg^T + bg) * (x Wu^T + bu), differentiable, and its
+  explicit forms `gated_linear_forward` / `gated_linear_backward`;
+* `quantize_mxfp4` / `dequantize_mxfp4` and `Mxfp4Matrix`, microscaled 4-bit matrices, with
+  `linear_mxfp4` and `gated_linear_mxfp4`, the same layers over 4-bit operands.
 """
 from __future__ import annotations
 
@@ -30,10 +38,13 @@ import ctypes
 import atexit
 import threading
 
+import dataclasses
+
 import torch
 
 from . import device as xd
 from . import sdk
+from ._native import Gated, lib
 
 _TF32X3 = 3
 _TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32: sdk.FP32,
@@ -120,6 +131,324 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         st = xd.bias_activation(y, y.shape[1], y.shape[1], y.shape[0], b, relu)
         _check(st, "xvram_b200_bias_activation")
     return y
+
+
+# ---------------------------------------------------------------- feed-forward operators
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+_FEED_TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32: sdk.FP32}
+
+
+def _activation(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)} (got {name!r})")
+    return ACTIVATIONS[name]
+
+
+def _on_device(device: torch.device):
+    """Makes `device` current for the library's calls, which use the current device."""
+    return torch.cuda.device(device)
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _aligned(x: torch.Tensor, ld: int) -> bool:
+    """Whether the tensor-core kernels can read x in place (float32 needs no alignment)."""
+    return x.dtype == torch.float32 or (x.data_ptr() % 16 == 0 and ld % 8 == 0)
+
+
+def _operand(x: torch.Tensor):
+    """(tensor, leading dimension, transposed): x itself where the kernels can read it, else a
+    copy whose rows are padded to 16 bytes."""
+    r, c = x.shape
+    s0, s1 = x.stride()
+    if s1 == 1 and s0 >= c and _aligned(x, s0):
+        return x, s0, 0
+    if s0 == 1 and s1 >= r and _aligned(x, s1):
+        return x, s1, 1
+    ld = (c + 7) // 8 * 8
+    y = torch.empty((r, ld), dtype=x.dtype, device=x.device)[:, :c]
+    y.copy_(x)
+    return y, ld, 0
+
+
+def _check_bias(b, h: int, like: torch.Tensor, name: str):
+    if b is None:
+        return None
+    if b.dtype != like.dtype or b.device != like.device or b.dim() != 1 or b.numel() != h:
+        raise ValueError(f"{name} must hold {h} values of the input's type on its device")
+    return b.contiguous()
+
+
+def _check_gated(x, w_gate, w_up) -> None:
+    if x.dtype not in _FEED_TYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+        raise TypeError("gated_linear supports float16, bfloat16 and float32 matrices of one type "
+                        f"(got {x.dtype}, {w_gate.dtype} and {w_up.dtype})")
+    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or \
+            x.shape[1] != w_gate.shape[1]:
+        raise ValueError(f"x (batch, in) and two (out, in) weights expected (got {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)} and {tuple(w_up.shape)})")
+    if x.shape[1] == 0:
+        raise ValueError("gated_linear needs at least one input feature")
+    if x.device.type != "cuda":
+        raise RuntimeError("gated_linear needs CUDA tensors (there is no CPU path)")
+    if w_gate.device != x.device or w_up.device != x.device:
+        raise ValueError("x and the weights must be on the same device")
+
+
+@dataclasses.dataclass
+class GatedSaved:
+    """What `gated_linear_backward` needs of a forward pass: the operands as the kernels read
+    them and the FP32 pre-activations."""
+    x: torch.Tensor
+    w_gate: torch.Tensor
+    w_up: torch.Tensor
+    pre_gate: torch.Tensor
+    pre_up: torch.Tensor
+    activation: str
+
+
+def _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act: int):
+    """The call's descriptor and the tensors it points to, which must outlive the call."""
+    xo, ldx, xt = _operand(x)
+    go, ldg, gt = _operand(w_gate)
+    uo, ldu, ut = _operand(w_up)
+    if gt != ut:  # one weight row-major, the other transposed: bring the latter to rows
+        if gt:
+            go, ldg, gt = _operand(w_gate.contiguous())
+        else:
+            uo, ldu, ut = _operand(w_up.contiguous())
+    d = Gated(ctypes.sizeof(Gated), _FEED_TYPES[x.dtype], act, xt, gt, 0, x.shape[0],
+              w_gate.shape[0], x.shape[1], xo.data_ptr(), go.data_ptr(), uo.data_ptr(), ldx, ldg,
+              ldu, _ptr(bias_gate), _ptr(bias_up), _ptr(pre_gate), _ptr(pre_up),
+              0 if pre_gate is None else pre_gate.stride(0), 0, 0, 0)
+    return d, (xo, go, uo)
+
+
+def _gated_workspace(d, backward: int, device: torch.device):
+    need = lib.xvram_b200_gated_workspace_bytes(ctypes.byref(d), backward)
+    if not need:
+        return None
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
+    d.workspace = (ws.data_ptr() + 255) // 256 * 256
+    d.workspace_bytes = need
+    return ws
+
+
+def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: bool):
+    act = _activation(activation)
+    _check_gated(x, w_gate, w_up)
+    m, h = x.shape[0], w_gate.shape[0]
+    bias_gate = _check_bias(bias_gate, h, x, "bias_gate")
+    bias_up = _check_bias(bias_up, h, x, "bias_up")
+    with _on_device(x.device):
+        out = torch.empty((m, h), dtype=x.dtype, device=x.device)
+        pre_gate = pre_up = None
+        if keep:
+            pre = torch.empty((2, m, (h + 3) // 4 * 4), dtype=torch.float32, device=x.device)
+            pre_gate, pre_up = pre[0], pre[1]
+        d, operands = _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act)
+        ws = _gated_workspace(d, 0, x.device)  # noqa: F841  (alive until the launch)
+        d.stream = _stream(x.device)
+        _check(lib.xvram_b200_gated_forward(ctypes.byref(d), out.data_ptr(), h),
+               "xvram_b200_gated_forward")
+    saved = GatedSaved(*operands, pre_gate, pre_up, activation) if keep else None
+    return out, saved
+
+
+def gated_linear_forward(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu"):
+    """(h, saved): the gated block's result and what `gated_linear_backward` needs.  For callers
+    that drive the backward pass themselves; autograd is not involved."""
+    with torch.no_grad():
+        return _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
+
+
+def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
+                          needs=(True, True, True, True, True)):
+    """Gradients (dx, dw_gate, dw_up, db_gate, db_up) of the block from dh = dL/dh; those that
+    `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
+    pre-activations are rounded to the type once, as the tensor cores' operands."""
+    x, w_gate, w_up = saved.x, saved.w_gate, saved.w_up
+    (m, k), h = x.shape, w_gate.shape[0]
+    if dh.shape != (m, h) or dh.dtype != x.dtype or dh.device != x.device:
+        raise ValueError(f"dh must be a ({m}, {h}) {x.dtype} tensor on {x.device}")
+    with torch.no_grad(), _on_device(x.device):
+        if dh.stride(1) != 1 or dh.stride(0) < h:
+            dh = dh.contiguous()
+        shapes = ((m, k), (h, k), (h, k), (h,), (h,))
+        grads = [torch.empty(s, dtype=x.dtype, device=x.device) if n else None
+                 for s, n in zip(shapes, needs)]
+        d, operands = _gated_desc(x, w_gate, w_up, None, None, saved.pre_gate, saved.pre_up,
+                                  _activation(saved.activation))
+        ws = _gated_workspace(d, 1, x.device)  # noqa: F841
+        d.stream = _stream(x.device)
+        dx, dwg, dwu, dbg, dbu = (_ptr(g) for g in grads)
+        _check(lib.xvram_b200_gated_backward(ctypes.byref(d), dh.data_ptr(), max(dh.stride(0), h),
+                                             dx, k, dwg, dwu, k, dbg, dbu),
+               "xvram_b200_gated_backward")
+    return tuple(grads)
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
+        out, saved = _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
+        ctx.save_for_backward(saved.x, saved.w_gate, saved.w_up, saved.pre_gate, saved.pre_up)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        saved = GatedSaved(*ctx.saved_tensors, ctx.activation)
+        return (*gated_linear_backward(dh, saved, ctx.needs_input_grad[:5]), None)
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                 bias_gate: torch.Tensor | None = None, bias_up: torch.Tensor | None = None,
+                 activation: str = "silu") -> torch.Tensor:
+    """act(x @ w_gate^T + bias_gate) * (x @ w_up^T + bias_up), x: (batch, in), weights:
+    (out, in), on CUDA tensors of one type (float16, bfloat16 or float32); activation: silu,
+    gelu, gelu_tanh, relu or sigmoid.  float16 / bfloat16 run as one tensor-core kernel with FP32
+    accumulation and one rounding, float32 in strict FP32.  Row-major and transposed operands
+    are read in place (16-bit ones where their base and leading dimension are multiples of 16
+    bytes; others are copied first).  Differentiable once in every tensor argument."""
+    tensors = (x, w_gate, w_up, bias_gate, bias_up)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _GatedLinear.apply(*tensors, activation)
+    return _gated_forward(*tensors, activation, False)[0]
+
+
+@dataclasses.dataclass(frozen=True)
+class Mxfp4Matrix:
+    """A (rows, cols) matrix in microscaled 4-bit floating point, stored as
+    include/xvram_b200.h lays it out: `codes` rows x ceil(cols / 32) x 16 bytes, `scales`
+    ceil(rows / 128) x ceil(cols / 128) tiles of 512 bytes, both contiguous uint8 CUDA tensors of
+    any shape.  Codes past the last column must be 0 and scales past the end not 255."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple[int, int]
+
+    def __post_init__(self):
+        rows, cols = self.shape
+        if rows < 0 or cols < 0:
+            raise ValueError("negative size")
+        for t, need, name in ((self.codes, rows * ((cols + 31) // 32) * 16, "codes"),
+                              (self.scales, ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
+                               "scales")):
+            if t.dtype != torch.uint8 or t.numel() != need or not t.is_contiguous() or \
+                    t.data_ptr() % 16:
+                raise ValueError(f"{name} of a ({rows}, {cols}) MXFP4 matrix must be {need} "
+                                 "contiguous bytes (uint8), 16-byte aligned")
+        if self.codes.device != self.scales.device:
+            raise ValueError("codes and scales must be on the same device")
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
+    """x (rows, cols; float16, bfloat16 or float32, CUDA) in MXFP4: blocks of 32 along each row
+    share the scale 2^(floor(log2 max|v|) - 2); elements are rounded to the nearest E2M1 value,
+    ties to even, saturating at 6 scales.  A block with a NaN or an infinity reads back as NaN."""
+    if x.dtype not in _FEED_TYPES:
+        raise TypeError(f"quantize_mxfp4 takes float16, bfloat16 or float32 (got {x.dtype})")
+    if x.dim() != 2:
+        raise ValueError("expected a 2-D tensor")
+    if x.device.type != "cuda":
+        raise RuntimeError("quantize_mxfp4 needs a CUDA tensor (there is no CPU path)")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("quantize_mxfp4 has no gradient: detach its input")
+    rows, cols = x.shape
+    with _on_device(x.device):
+        if x.stride(1) != 1 or x.stride(0) < cols:
+            x = x.contiguous()
+        codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(((rows + 127) // 128, (cols + 127) // 128, 512), dtype=torch.uint8,
+                             device=x.device)
+        _check(lib.xvram_b200_mxfp4_quantize(_FEED_TYPES[x.dtype], rows, cols, x.data_ptr(),
+                                             max(x.stride(0), cols), codes.data_ptr(),
+                                             scales.data_ptr(), _stream(x.device)),
+               "xvram_b200_mxfp4_quantize")
+    return Mxfp4Matrix(codes, scales, (rows, cols))
+
+
+def dequantize_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of q as a (rows, cols) tensor (exact in float32, rounded once in float16 and
+    bfloat16)."""
+    if dtype not in _FEED_TYPES:
+        raise TypeError(f"dequantize_mxfp4 gives float16, bfloat16 or float32 (got {dtype})")
+    if q.device.type != "cuda":
+        raise RuntimeError("dequantize_mxfp4 needs a CUDA matrix (there is no CPU path)")
+    rows, cols = q.shape
+    with _on_device(q.device):
+        out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+        _check(lib.xvram_b200_mxfp4_dequantize(_FEED_TYPES[dtype], rows, cols, q.codes.data_ptr(),
+                                               q.scales.data_ptr(), out.data_ptr(), cols,
+                                               _stream(q.device)), "xvram_b200_mxfp4_dequantize")
+    return out
+
+
+def _mxfp4_input(x, dtype, weights, what: str):
+    """(MXFP4 input, result type) of a product, its arguments checked."""
+    given = x.dtype if isinstance(x, torch.Tensor) else torch.float32
+    dtype = given if dtype is None else dtype
+    if dtype not in _FEED_TYPES or (isinstance(x, torch.Tensor) and x.dtype not in _FEED_TYPES):
+        raise TypeError(f"{what} supports float16, bfloat16 and float32 (got {given} to {dtype})")
+    if len(x.shape) != 2 or any(not isinstance(w, Mxfp4Matrix) or w.shape[1] != x.shape[1] or
+                                w.shape != weights[0].shape for w in weights):
+        raise ValueError(f"{what} takes x (batch, in) and MXFP4 weights (out, in)")
+    if x.shape[1] == 0:
+        raise ValueError(f"{what} needs at least one input feature")
+    if x.device.type != "cuda" or any(w.device != x.device for w in weights):
+        raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
+    return (quantize_mxfp4(x) if isinstance(x, torch.Tensor) else x), dtype
+
+
+def linear_mxfp4(x, weight: Mxfp4Matrix, bias: torch.Tensor | None = None, relu: bool = False,
+                 dtype: torch.dtype | None = None) -> torch.Tensor:
+    """Q(x) @ weight^T (+ bias) (then ReLU) on the block-scaled tensor-core product of two MXFP4
+    operands, FP32 accumulation, rounded once.  x: (batch, in), a float tensor that is quantised
+    here or an Mxfp4Matrix; weight: (out, in).  The result (and the bias) has `dtype`: x's type by
+    default, float32 for an Mxfp4Matrix.  Inference only: no gradient."""
+    xq, dtype = _mxfp4_input(x, dtype, (weight,), "linear_mxfp4")
+    m, n, k = x.shape[0], weight.shape[0], x.shape[1]
+    with _on_device(xq.device):
+        out = torch.empty((m, n), dtype=dtype, device=xq.device)
+        bias = _check_bias(bias, n, out, "bias")
+        _check(lib.xvram_b200_mxfp4_linear(_FEED_TYPES[dtype], m, n, k, xq.codes.data_ptr(),
+                                           xq.scales.data_ptr(), weight.codes.data_ptr(),
+                                           weight.scales.data_ptr(), _ptr(bias), 1 if relu else 0,
+                                           out.data_ptr(), n, _stream(xq.device)),
+               "xvram_b200_mxfp4_linear")
+    return out
+
+
+def gated_linear_mxfp4(x, w_gate: Mxfp4Matrix, w_up: Mxfp4Matrix,
+                       bias_gate: torch.Tensor | None = None, bias_up: torch.Tensor | None = None,
+                       activation: str = "silu", dtype: torch.dtype | None = None) -> torch.Tensor:
+    """`gated_linear` over MXFP4 operands, with `linear_mxfp4`'s input and types: both products,
+    the biases, the activation and the product of the two in one kernel.  No gradient."""
+    act = _activation(activation)
+    xq, dtype = _mxfp4_input(x, dtype, (w_gate, w_up), "gated_linear_mxfp4")
+    m, h, k = x.shape[0], w_gate.shape[0], x.shape[1]
+    with _on_device(xq.device):
+        out = torch.empty((m, h), dtype=dtype, device=xq.device)
+        bias_gate = _check_bias(bias_gate, h, out, "bias_gate")
+        bias_up = _check_bias(bias_up, h, out, "bias_up")
+        _check(lib.xvram_b200_mxfp4_gated(_FEED_TYPES[dtype], act, m, h, k, xq.codes.data_ptr(),
+                                          xq.scales.data_ptr(), w_gate.codes.data_ptr(),
+                                          w_gate.scales.data_ptr(), w_up.codes.data_ptr(),
+                                          w_up.scales.data_ptr(), _ptr(bias_gate), _ptr(bias_up),
+                                          out.data_ptr(), h, _stream(xq.device)),
+               "xvram_b200_mxfp4_gated")
+    return out
 
 
 class HostGemm:
