@@ -71,3 +71,10 @@ def test_gradients(kind, shape):
 @pytest.mark.parametrize("kind", TYPES)
 def test_gradients_of_each_activation(kind, act):
     check_gradients(problem(kind, 70, 144, 40, 30), act, fu.normal((70, 144), kind, 31))
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+def test_more_tiles_than_the_gpu_holds(kind):
+    """Each resident CTA pair walks several tiles, in the forward and in both gradient products."""
+    m, h, k = 2200, 1500, 2050
+    check_gradients(problem(kind, m, h, k, 40), "gelu_tanh", fu.normal((m, h), kind, 41))

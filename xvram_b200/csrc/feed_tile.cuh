@@ -262,10 +262,147 @@ __device__ __forceinline__ void add_bias(const void* bias, int col, int n, float
       v[i] += to_float(b[col + i]);
 }
 
+// 16 output columns from `col` on of this thread's row: TMEM columns c0.. (and 128 + c0.. for the
+// up projection) to the result.  Collective over the warp.
+template <Epilogue E, class T>
+__device__ __forceinline__ void epilogue_chunk(const Params& p, uint32_t t_row, int c0, int col,
+                                               int row, T* out) {
+  constexpr bool kFast = sizeof(T) == 2;
+  if (col >= p.n)
+    return; // uniform over the warp
+  __syncwarp();
+  uint32_t r0[16], r1[16];
+  tc::tmem_ld16(t_row + c0, r0);
+  if constexpr (E == Epilogue::gated)
+    tc::tmem_ld16(t_row + 128 + c0, r1);
+  tc::tmem_wait_ld();
+  if (row >= p.m)
+    return;
+  float v[16], w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    v[i] = __uint_as_float(r0[i]);
+  add_bias<T>(p.bias0, col, p.n, v);
+  if constexpr (E == Epilogue::gated) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      w[i] = __uint_as_float(r1[i]);
+    add_bias<T>(p.bias1, col, p.n, w);
+    if (p.save_gate) {
+      store_row(p.save_gate + static_cast<long long>(row) * p.lds, col, p.n, true, v);
+      store_row(p.save_up + static_cast<long long>(row) * p.lds, col, p.n, true, w);
+    }
+    gate<kFast>(p.act, v, w);
+  } else if (p.relu) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      v[i] = act_of<kRelu, kFast>(v[i]);
+  }
+  store_row(out, col, p.n, p.vec_out != 0, v);
+}
+
+// A warp's half of an accumulator to registers: the gated form's 64 gate and 64 up columns, or the
+// plain form's 128 columns.  Collective over the warp.
+template <Epilogue E>
+__device__ __forceinline__ void load_accumulator(uint32_t t_row, int half, float (&v)[128]) {
+  uint32_t r[128 / 16][16];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = E == Epilogue::gated ? (i < 4 ? 64 * half + 16 * i : 128 + 64 * half + 16 * (i - 4))
+                                       : 128 * half + 16 * i;
+    tc::tmem_ld16(t_row + c, r[i]);
+  }
+  tc::tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 128; ++i)
+    v[i] = __uint_as_float(r[i / 16][i % 16]);
+}
+
+// A warp's 32 rows x 128 bytes of results, row per lane, to global memory in whole lines:
+// through `block` (shared memory, 16-byte chunks swizzled by the row), then 8 lanes per row.
+constexpr int kStageBlock = 32 * 128;
+template <class T, int N>
+__device__ __forceinline__ void store_block(unsigned char* block, const float (&v)[N], int from,
+                                            T* out, long long ld, int row0, int col, int m, int n,
+                                            bool vec) {
+  constexpr int per = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    alignas(16) T t[per];
+#pragma unroll
+    for (int j = 0; j < per; ++j)
+      t[j] = from_float<T>(v[from + c * per + j]);
+    *reinterpret_cast<uint4*>(block + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+        *reinterpret_cast<const uint4*>(t);
+  }
+  __syncwarp();
+  const int c = lane & 7, cc = col + c * per;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    const uint4 raw = *reinterpret_cast<const uint4*>(block + r * 128 + ((c ^ (r & 7)) * 16));
+    if (row0 + r < m) {
+      T* dst = out + static_cast<long long>(row0 + r) * ld + cc;
+      if (vec && cc + per <= n) {
+        *reinterpret_cast<uint4*>(dst) = raw;
+      } else {
+        const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+        for (int j = 0; j < per; ++j)
+          if (cc + j < n)
+            dst[j] = t[j];
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// The loaded accumulator half to results: 64 gated or 128 plain columns from `col` on of the
+// warp's rows row0...
+template <Epilogue E, class T>
+__device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], int row0, int col,
+                                            T* out, unsigned char* block) {
+  constexpr int kBlockCols = 128 / sizeof(T); // columns of a stored block
+  if (col >= p.n || row0 >= p.m)
+    return; // uniform over the warp
+  if constexpr (E == Epilogue::gated) {
+    float g[64], u[64];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      g[i] = v[i];
+      u[i] = v[64 + i];
+    }
+    add_bias<T>(p.bias0, col, p.n, g);
+    add_bias<T>(p.bias1, col, p.n, u);
+    if (p.save_gate) {
+#pragma unroll
+      for (int i = 0; i < 64; i += 32) {
+        store_block(block, g, i, p.save_gate, p.lds, row0, col + i, p.m, p.n, true);
+        store_block(block, u, i, p.save_up, p.lds, row0, col + i, p.m, p.n, true);
+      }
+    }
+    gate<sizeof(T) == 2>(p.act, g, u);
+#pragma unroll
+    for (int i = 0; i < 64; i += kBlockCols)
+      store_block(block, g, i, out, p.ldo, row0, col + i, p.m, p.n, p.vec_out != 0);
+  } else {
+    add_bias<T>(p.bias0, col, p.n, v);
+    if (p.relu) {
+#pragma unroll
+      for (int i = 0; i < 128; ++i)
+        v[i] = act_of<kRelu, true>(v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 128; i += kBlockCols)
+      store_block(block, v, i, out, p.ldo, row0, col + i, p.m, p.n, p.vec_out != 0);
+  }
+}
+
 template <Kind K, Epilogue E, class T>
 __global__ void __launch_bounds__(kThreads, 1)
     feed_tile_kernel(const __grid_constant__ Maps maps, const Params p) {
-  constexpr bool kFast = sizeof(T) == 2;
   constexpr int kStageBytes = stage_bytes<K>();
   constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
   constexpr int kElems = K == Kind::f16 ? 64 : 128; // map elements per 128-byte row
@@ -432,39 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (__all_sync(0xffffffffu, ok && !*abort_flag)) {
       const uint32_t t_row = tmem + (static_cast<uint32_t>(32 * quad) << 16);
       T* out = static_cast<T*>(p.out[batch]) + static_cast<long long>(row) * p.ldo;
-      for (int c0 = half * (kTileN / 2); c0 < (half + 1) * (kTileN / 2); c0 += 16) {
-        const int col = n0 + c0;
-        if (col >= p.n)
-          break; // uniform over the warp
-        uint32_t r0[16], r1[16];
-        float v[16], w[16];
-        tc::tmem_ld16(t_row + c0, r0);
-        if constexpr (E == Epilogue::gated)
-          tc::tmem_ld16(t_row + 128 + c0, r1);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          v[i] = __uint_as_float(r0[i]);
-        if (row < p.m) {
-          add_bias<T>(p.bias0, col, p.n, v);
-          if constexpr (E == Epilogue::gated) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              w[i] = __uint_as_float(r1[i]);
-            add_bias<T>(p.bias1, col, p.n, w);
-            if (p.save_gate) {
-              store_row(p.save_gate + static_cast<long long>(row) * p.lds, col, p.n, true, v);
-              store_row(p.save_up + static_cast<long long>(row) * p.lds, col, p.n, true, w);
-            }
-            gate<kFast>(p.act, v, w);
-          } else if (p.relu) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              v[i] = act_of<kRelu, kFast>(v[i]);
-          }
-          store_row(out, col, p.n, p.vec_out != 0, v);
-        }
-      }
+      for (int c0 = half * (kTileN / 2); c0 < (half + 1) * (kTileN / 2); c0 += 16)
+        epilogue_chunk<E, T>(p, t_row, c0, n0 + c0, row, out);
     }
     tc::fence_before();
   }

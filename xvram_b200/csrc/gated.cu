@@ -15,6 +15,8 @@
 // FP32 runs on the strict FP32 GEMM kernel.  There the product takes 2 k / 3 FMAs per float
 // the elementwise passes move: at k = 1024 and more the passes are under 3% of the time, so they
 // stay separate kernels.
+#include "feed_pair.cuh"
+#include "feed_rows.cuh"
 #include "feed_tile.cuh"
 #include "kernels.hpp"
 
@@ -235,6 +237,21 @@ Params base_params(bool bf16, int m, int n, int k_tiles, bool a_mn, bool b_mn, i
   return p;
 }
 
+// The pair kernel above one row tile, with 512-row tiles where their waves cost less: one runs in
+// 1.85 times a 256-row tile's time (8192 x 4096 x 8192, seconds of it back to back under the
+// power cap: 832 us against 859; 2048 rows, 4 waves against 7: 231 against 222).
+template <Epilogue E, class T>
+cudaError_t launch_16(const Maps& maps, Params p, bool bf16, cudaStream_t stream) {
+  if (p.m <= 128)
+    return launch_tiles<Kind::f16, E, T>(maps, p, stream);
+  p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 256, 256);
+  const long long pairs = tc::sm_count() / 2, cols = static_cast<long long>(p.batches) * p.tiles_n;
+  const long long one = (cols * ((p.m + 255) / 256) + pairs - 1) / pairs;
+  const long long two = (cols * ((p.m + 511) / 512) + pairs - 1) / pairs;
+  return 1.85 * two < one ? launch_pairs<E, T, 2>(maps, p, stream)
+                          : launch_pairs<E, T, 1>(maps, p, stream);
+}
+
 template <class T>
 cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStream_t stream) {
   constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
@@ -254,7 +271,7 @@ cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStre
   p.save_gate = q.pre_gate;
   p.save_up = q.pre_up;
   p.lds = q.ld_pre;
-  return launch_tiles<Kind::f16, Epilogue::gated, T>(maps, p, stream);
+  return launch_16<Epilogue::gated, T>(maps, p, bf16, stream);
 }
 
 template <class T>
@@ -288,7 +305,7 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[0] = p.out[1] = d.dx;
     p.ldo = d.lddx;
     p.vec_out = d.lddx % 8 == 0 && aligned16(d.dx);
-    if (cudaError_t e = launch_tiles<Kind::f16, Epilogue::plain, T>(maps, p, stream);
+    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, bf16, stream);
         e != cudaSuccess)
       return e;
   }
@@ -308,11 +325,58 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[1] = d.dw_up;
     p.ldo = d.ld_dw;
     p.vec_out = d.ld_dw % 8 == 0 && aligned16(p.out[0]) && aligned16(p.out[1]);
-    if (cudaError_t e = launch_tiles<Kind::f16, Epilogue::plain, T>(maps, p, stream);
+    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, bf16, stream);
         e != cudaSuccess)
       return e;
   }
   return cudaSuccess;
+}
+
+// ---------------------------------------------------------------- few rows
+template <class T>
+cudaError_t forward_rows(const GatedProblem& q, void* out, long long ldo, cudaStream_t stream) {
+  RowsParams p{};
+  p.x = q.x;
+  p.w_gate = q.w_gate;
+  p.w_up = q.w_up;
+  p.ldx = q.ldx;
+  p.ld_gate = q.ld_gate;
+  p.ld_up = q.ld_up;
+  p.bias_gate = q.bias_gate;
+  p.bias_up = q.bias_up;
+  p.out = out;
+  p.ldo = ldo;
+  p.save_gate = q.pre_gate;
+  p.save_up = q.pre_up;
+  p.lds = q.ld_pre;
+  p.m = q.m;
+  p.h = q.h;
+  p.k = q.k;
+  p.act = q.act;
+  constexpr long long per = 16 / sizeof(T);
+  const bool vec = aligned16(q.x) && aligned16(q.w_gate) && aligned16(q.w_up) &&
+                   q.ldx % per == 0 && q.ld_gate % per == 0 && q.ld_up % per == 0;
+  return vec ? launch_rows<T, static_cast<int>(per)>(p, stream) : launch_rows<T, 1>(p, stream);
+}
+
+// Whether the forward runs on the few-rows kernel.  It reads each weight once per 8 rows of x and
+// sustains about 20 TFLOP/s of FP32 FMAs; measured against the tile kernels (device time,
+// weights larger than L2 rotated):
+//   FP32, 4096 inputs, 8192 features: 46 us for 2 rows (5.8 TB/s), 431 for 64, 865 for 128, against
+//   548 us for the FFMA kernel, whose waves of 148 128 x 128 tiles take 0.066 us per input whatever
+//   m is; 1024 x 2048: 62 us for 128 rows against 136.  4 m h k / 20 TFLOP/s is below the two GEMMs'
+//   2 x 0.066 us k waves while m h < 640k waves.
+//   BF16, same sizes: 25 and 3.9 us for one row, 34 and 5.0 for 4, 64 and 6.3 for 8, against the
+//   tensor cores' 35-40 and 11.
+bool few_rows(const GatedProblem& q) {
+  if (q.x_transposed || q.w_transposed)
+    return false;
+  if (q.type != GatedType::f32)
+    return q.m <= 4;
+  if (q.m > 512)
+    return false;
+  const long long tiles = ((q.h + 127ll) / 128) * ((q.m + 127) / 128), sms = tc::sm_count();
+  return static_cast<long long>(q.m) * q.h < 640000 * ((tiles + sms - 1) / sms);
 }
 
 // ---------------------------------------------------------------- FP32 on the FFMA kernel
@@ -411,6 +475,8 @@ uint64_t gated_workspace_bytes(const GatedProblem& q, bool backward) {
   if (q.m <= 0 || q.h <= 0 || q.k <= 0)
     return 0;
   const uint64_t m = q.m, h = q.h;
+  if (!backward && few_rows(q))
+    return 0;
   if (q.type == GatedType::f32) {
     const uint64_t pair = 2 * up(m * up(h, 4) * 4, 256);
     return backward ? pair + gated_partial_bytes(q.m, q.h) + sgemm_scratch_bwd(q)
@@ -424,6 +490,13 @@ cudaError_t gated_forward(const GatedProblem& q, void* out, long long ldo, void*
   const uint64_t need = gated_workspace_bytes(q, false);
   if (workspace_bytes < need || (need && (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return cudaErrorInvalidValue;
+  if (few_rows(q)) {
+    switch (q.type) {
+    case GatedType::f16: return forward_rows<__half>(q, out, ldo, stream);
+    case GatedType::bf16: return forward_rows<__nv_bfloat16>(q, out, ldo, stream);
+    default: return forward_rows<float>(q, out, ldo, stream);
+    }
+  }
   switch (q.type) {
   case GatedType::f16: return forward_16<__half>(q, out, ldo, stream);
   case GatedType::bf16: return forward_16<__nv_bfloat16>(q, out, ldo, stream);

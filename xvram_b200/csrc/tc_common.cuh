@@ -78,6 +78,14 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         : "memory");
 }
 
+// mma_commit of a pair's leader to the barriers at this shared::cta offset in both CTAs.
+__device__ __forceinline__ void mma_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::"
+               "cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+
 // D[tmem] (+)= A[smem] B[smem]^T of 16-bit elements, FP32 accumulation.
 template <int PAIR>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,

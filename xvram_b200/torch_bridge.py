@@ -167,6 +167,8 @@ def _operand(x: torch.Tensor):
     copy whose rows are padded to 16 bytes."""
     r, c = x.shape
     s0, s1 = x.stride()
+    if r == 1 and s1 == 1:  # one row's stride is never used
+        s0 = (c + 7) // 8 * 8
     if s1 == 1 and s0 >= c and _aligned(x, s0):
         return x, s0, 0
     if s0 == 1 and s1 >= r and _aligned(x, s1):
