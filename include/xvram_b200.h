@@ -455,18 +455,35 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_quantize(
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
     uint32_t data_type, int64_t rows, int64_t cols, uint64_t codes, uint64_t scales, uint64_t dst,
     int64_t ldd, uint64_t stream);
-/* out (m x n) = x W^T (+ bias) (then ReLU): x m x k and W n x k, both MXFP4, on the block-scaled
- * tensor-core MMA with FP32 accumulation; out and bias (n values, or 0) of out_type. */
-XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_linear(
-    uint32_t out_type, int64_t m, int64_t n, int64_t k, uint64_t x_codes, uint64_t x_scales,
-    uint64_t w_codes, uint64_t w_scales, uint64_t bias, uint32_t activation, uint64_t out,
-    int64_t ld_out, uint64_t stream);
-/* The gated block over MXFP4 operands: out (m x h) = act(x Wg^T + bg) * (x Wu^T + bu). */
-XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_gated(
-    uint32_t out_type, uint32_t activation, int64_t m, int64_t h, int64_t k, uint64_t x_codes,
-    uint64_t x_scales, uint64_t gate_codes, uint64_t gate_scales, uint64_t up_codes,
-    uint64_t up_scales, uint64_t bias_gate, uint64_t bias_up, uint64_t out, int64_t ld_out,
-    uint64_t stream);
+/*
+ * Products of MXFP4 matrices on the block-scaled tensor-core MMA, FP32 accumulation, one
+ * rounding to out_type:
+ *   linear: out (m x n) = x W^T (+ bias) (then ReLU), W = (w_codes[0], w_scales[0]), bias[0];
+ *   gated:  out (m x n) = act(x W0^T + bias[0]) * (x W1^T + bias[1]).
+ * x (m x k): with x set, rows of `x_type` values, ldx elements apart, which are quantised into
+ * x_codes and x_scales first (caller's memory, as xvram_b200_mxfp4_bytes says; it may be reused
+ * once the call's work on `stream` is done); with x = 0, x_codes and x_scales as they are.  Biases
+ * (0 for none) hold n values of out_type.
+ */
+typedef struct xvram_b200_mxfp4_product_v1 {
+  uint32_t struct_size; /* sizeof(xvram_b200_mxfp4_product_v1) */
+  uint32_t x_type, out_type; /* XVRAM_DATA_FP16, _BF16 or _FP32 */
+  uint32_t activation; /* linear: XVRAM_B200_ACTIVATION_*; gated: XVRAM_B200_GATE_* */
+  int64_t m, n, k; /* m and n >= 0, k >= 1 */
+  uint64_t x;
+  int64_t ldx;
+  uint64_t x_codes, x_scales;
+  uint64_t w_codes[2], w_scales[2];
+  uint64_t bias[2];
+  uint64_t out;
+  int64_t ld_out;
+  uint64_t stream;
+} xvram_b200_mxfp4_product_v1;
+
+XVRAM_B200_API xvram_status XVRAM_CALL
+xvram_b200_mxfp4_linear(const xvram_b200_mxfp4_product_v1* product);
+XVRAM_B200_API xvram_status XVRAM_CALL
+xvram_b200_mxfp4_gated(const xvram_b200_mxfp4_product_v1* product);
 
 /* Extra state of the compat adapter's runtime (not in the reference telemetry). */
 typedef struct xvram_b200_runtime_info_v1 {

@@ -98,6 +98,16 @@ class Gated(C.Structure):
                 ("ld_pre", i64), ("workspace", u64), ("workspace_bytes", u64), ("stream", u64)]
 
 
+class Mxfp4Product(C.Structure):
+    """xvram_b200_mxfp4_product_v1 (include/xvram_b200.h)."""
+
+    _fields_ = [("struct_size", u32), ("x_type", u32), ("out_type", u32), ("activation", u32),
+                ("m", i64), ("n", i64), ("k", i64), ("x", u64), ("ldx", i64),
+                ("x_codes", u64), ("x_scales", u64), ("w_codes0", u64), ("w_codes1", u64),
+                ("w_scales0", u64), ("w_scales1", u64), ("bias0", u64), ("bias1", u64),
+                ("out", u64), ("ld_out", i64), ("stream", u64)]
+
+
 def _load() -> C.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(
@@ -183,12 +193,9 @@ def _load() -> C.CDLL:
     lib.xvram_b200_mxfp4_quantize.restype = u32
     lib.xvram_b200_mxfp4_dequantize.argtypes = [u32, i64, i64, u64, u64, u64, i64, u64]
     lib.xvram_b200_mxfp4_dequantize.restype = u32
-    lib.xvram_b200_mxfp4_linear.argtypes = [u32, i64, i64, i64, u64, u64, u64, u64, u64, u32, u64,
-                                            i64, u64]
-    lib.xvram_b200_mxfp4_linear.restype = u32
-    lib.xvram_b200_mxfp4_gated.argtypes = [u32, u32, i64, i64, i64, u64, u64, u64, u64, u64, u64,
-                                           u64, u64, u64, i64, u64]
-    lib.xvram_b200_mxfp4_gated.restype = u32
+    for fn in (lib.xvram_b200_mxfp4_linear, lib.xvram_b200_mxfp4_gated):
+        fn.argtypes = [C.POINTER(Mxfp4Product)]
+        fn.restype = u32
     lib.xvram_b200_digest_bench.argtypes = [vp, u64, u64, C.POINTER(u64)]
     lib.xvram_b200_digest_bench.restype = None
     lib.xvram_b200_digest_compat.argtypes = [vp, u64, C.POINTER(u64)]

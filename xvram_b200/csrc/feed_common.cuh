@@ -1,4 +1,5 @@
-// feed_tile.cuh -- the tensor-core tile kernel of the feed-forward operators.
+// feed_common.cuh -- what the tensor-core kernels of the feed-forward operators share:
+// operand geometry, instruction descriptors, activations and the epilogue.
 //
 //   D[m, n] = sum_k A[m, k] B[n, k]                       FP32 accumulation in TMEM
 //   gated:  out[m, h] = act(D[m, h] + b0[h]) * (D'[m, h] + b1[h]), D from B0 and D' from B1
@@ -7,17 +8,10 @@
 // Operands are 16-bit floats (kind::f16) or MXFP4 codes with their block scales (kind::mxf4).
 // The stage geometry is the same for both: 128 bytes of K per operand row and stage, 128-byte
 // swizzle, four MMAs of 32 bytes of K.  16-bit operands may also be stored M-/N-major
-// (contiguous along their rows); MXFP4 operands are K-major.
-//
-// One CTA holds 128 rows of A and two 128-row parts of B, so its accumulator is 128 x 256: for the gated
-// form part 0 is the gate's weight rows and part 1 the up projection's rows of the same
-// features, so each thread of the epilogue finds both pre-activations of an output in its own
-// TMEM lane and the product needs no exchange.  The plain form's parts are neighbouring rows
-// of one B.
-//
-//   warp 0      one lane: TMA loads of a stage's operands (and bulk copies of its scales);
-//   warp 1      one lane: copies the scales to TMEM, issues the MMAs, commits;
-//   warps 2..9  epilogue, two warps per TMEM lane quarter splitting the columns.
+// (contiguous along their rows); MXFP4 operands are K-major.  Accumulators have 256 columns
+// from two 128-row parts of B: for the gated form the gate's and the up projection's rows of
+// the same 128 features, so that each epilogue thread finds both pre-activations of an output in
+// its own TMEM lane and the product needs no exchange; for the plain form neighbouring rows.
 //
 // All waits are bounded: a wait that runs out sets a bit of the kernel error word, the CTA
 // stops issuing, frees its TMEM and returns.
@@ -32,7 +26,8 @@ namespace xvram::feed {
 
 constexpr int kThreads = 320; // producer, MMA, 8 epilogue warps
 constexpr uint32_t kPart = 128 * 128;        // bytes of one 128-row operand part of a stage
-constexpr uint32_t kScaleBytes = 3 * 1024;   // A's and both B parts' scales of a stage
+constexpr uint32_t kScaleTile = 1024;        // bytes of a 128-row part's scales of a stage
+constexpr uint32_t kScaleBytes = 3 * kScaleTile; // A's and both B parts'
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kScaleCol = 256;          // first TMEM column of the MXFP4 scales
 constexpr uint32_t kScaleCols = 24;          // per stage: A 2 x 4, B 2 x 8
@@ -47,22 +42,19 @@ enum Act : int { kSilu = 0, kGelu = 1, kGeluTanh = 2, kRelu = 3, kSigmoid = 4 };
 // 8 an epilogue gave up waiting.
 static __device__ unsigned int feed_error = 0;
 
+// Operands of up to two products that share an accumulator or a launch, and MXFP4 scales.
 struct Maps {
-  CUtensorMap a[2], b[2];
+  CUtensorMap a[2], b[2], scale_a, scale_b[2];
 };
 
 struct Params {
   int m, n;               // output rows and columns
   int k_tiles, k_split;   // stages in all; stages of the first operand pair (a[0], b[0])
-  int last_steps;         // MMA steps of the last stage
   int tiles_m, tiles_n, batches;
   int a_mn, b_mn;         // 16-bit operands stored M-/N-major
   int act, relu;
-  int vec_out;            // outputs (and biases) allow 16-byte accesses
+  int vec_out;            // output rows allow 16-byte accesses
   uint32_t idesc;
-  // MXFP4: scale tiles of 512 bytes (128 rows x 4 blocks), `scale_k` of them per row tile
-  const unsigned char *scale_a, *scale_b[2];
-  int scale_k, scale_rows_b;
   const void *bias0, *bias1;
   void* out[2];           // by batch
   long long ldo;
@@ -70,16 +62,6 @@ struct Params {
   long long lds;
   unsigned long long timeout_ns;
 };
-
-template <Kind K>
-__host__ __device__ constexpr int stage_bytes() {
-  return 3 * kPart + (K == Kind::mxf4 ? kScaleBytes : 0);
-}
-constexpr int kStages = 4;
-template <Kind K>
-__host__ __device__ constexpr int smem_bytes() {
-  return kStages * stage_bytes<K>() + 1024 + 256;
-}
 
 // Instruction descriptors.  16-bit: D F32, operand format (0 FP16, 1 BF16), majors, N and M.
 inline uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn, int m, int n) {
@@ -93,33 +75,76 @@ inline uint32_t idesc_mxf4(int m, int n) {
          (static_cast<uint32_t>(m >> 7) << 27);
 }
 
+template <int PAIR>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                          uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile("{\n"
-               "  .reg .pred p;\n"
-               "  setp.ne.b32 p, %6, 0;\n"
-               "  tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, "
-               "[%4], [%5], p;\n"
-               "}\n" ::"r"(d),
-               "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-               : "memory");
+  if constexpr (PAIR == 2)
+    asm volatile("{\n"
+                 "  .reg .pred p;\n"
+                 "  setp.ne.b32 p, %6, 0;\n"
+                 "  tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, "
+                 "%3, [%4], [%5], p;\n"
+                 "}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+                 : "memory");
+  else
+    asm volatile("{\n"
+                 "  .reg .pred p;\n"
+                 "  setp.ne.b32 p, %6, 0;\n"
+                 "  tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, "
+                 "%3, [%4], [%5], p;\n"
+                 "}\n" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+                 : "memory");
 }
 
 // One scale tile (128 rows x 4 blocks, 32 x 16 bytes) from shared memory to 4 TMEM columns,
-// replicated over the four lane quarters.  Unswizzled: 8-row groups are 128 bytes apart.
+// replicated over the four lane quarters; for a pair in both CTAs, each from its own shared
+// memory.  Unswizzled: 8-row groups are 128 bytes apart.
+template <int PAIR>
 __device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr) {
   const uint64_t desc = static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | (1ull << 16) |
                         (8ull << 32) | (1ull << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc)
-               : "memory");
+  if constexpr (PAIR == 2)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc)
+                 : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc)
+                 : "memory");
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, "
-               "[%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+// The four MMAs of a 16-bit stage.
+template <int PAIR>
+__device__ __forceinline__ void stage_f16(const Params& p, uint32_t d, uint32_t a, uint32_t b,
+                                          bool first) {
+  const uint64_t sa = p.a_mn ? 128 : 2, sb = p.b_mn ? 128 : 2; // 16-byte units per step
+  const uint64_t da = p.a_mn ? tc::desc_mnmajor(a) : tc::desc_kmajor(a);
+  const uint64_t db = p.b_mn ? tc::desc_mnmajor(b) : tc::desc_kmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk)
+    tc::mma_f16<PAIR>(d, da + kk * sa, db + kk * sb, p.idesc, (first && kk == 0) ? 0u : 1u);
+}
+
+// The scale copies and the four MMAs of an MXFP4 stage.  The scales of a stage have TMEM
+// columns of their own, which the stage's next use overwrites only after its MMAs have completed
+// (the stage's barrier says so).  K past the end has zero codes and zero (2^-127) scales.
+template <int PAIR>
+__device__ __forceinline__ void stage_mxf4(const Params& p, uint32_t d, uint32_t a, uint32_t b,
+                                           uint32_t scales, uint32_t sf, bool first) {
+  const uint32_t sfa = sf, sfb = sf + 8;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    copy_scales<PAIR>(sfa + 4 * g, scales + 512 * g);
+    copy_scales<PAIR>(sfb + 8 * g, scales + kScaleTile + 512 * g);
+    copy_scales<PAIR>(sfb + 8 * g + 4, scales + 2 * kScaleTile + 512 * g);
+  }
+  const uint64_t da = tc::desc_kmajor(a), db = tc::desc_kmajor(b);
+#pragma unroll
+  for (int kk = 0; kk < 4; ++kk) {
+    const uint32_t id = (kk & 1) * 2; // byte of the scale column for this step
+    mma_mxf4<PAIR>(d, da + kk * 2, db + kk * 2, p.idesc | (id << 4) | (id << 29),
+                   sfa + 4 * (kk >> 1), sfb + 8 * (kk >> 1), (first && kk == 0) ? 0u : 1u);
+  }
 }
 
 // ---------------------------------------------------------------- activations
@@ -262,45 +287,6 @@ __device__ __forceinline__ void add_bias(const void* bias, int col, int n, float
       v[i] += to_float(b[col + i]);
 }
 
-// 16 output columns from `col` on of this thread's row: TMEM columns c0.. (and 128 + c0.. for the
-// up projection) to the result.  Collective over the warp.
-template <Epilogue E, class T>
-__device__ __forceinline__ void epilogue_chunk(const Params& p, uint32_t t_row, int c0, int col,
-                                               int row, T* out) {
-  constexpr bool kFast = sizeof(T) == 2;
-  if (col >= p.n)
-    return; // uniform over the warp
-  __syncwarp();
-  uint32_t r0[16], r1[16];
-  tc::tmem_ld16(t_row + c0, r0);
-  if constexpr (E == Epilogue::gated)
-    tc::tmem_ld16(t_row + 128 + c0, r1);
-  tc::tmem_wait_ld();
-  if (row >= p.m)
-    return;
-  float v[16], w[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    v[i] = __uint_as_float(r0[i]);
-  add_bias<T>(p.bias0, col, p.n, v);
-  if constexpr (E == Epilogue::gated) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      w[i] = __uint_as_float(r1[i]);
-    add_bias<T>(p.bias1, col, p.n, w);
-    if (p.save_gate) {
-      store_row(p.save_gate + static_cast<long long>(row) * p.lds, col, p.n, true, v);
-      store_row(p.save_up + static_cast<long long>(row) * p.lds, col, p.n, true, w);
-    }
-    gate<kFast>(p.act, v, w);
-  } else if (p.relu) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      v[i] = act_of<kRelu, kFast>(v[i]);
-  }
-  store_row(out, col, p.n, p.vec_out != 0, v);
-}
-
 // A warp's half of an accumulator to registers: the gated form's 64 gate and 64 up columns, or the
 // plain form's 128 columns.  Collective over the warp.
 template <Epilogue E>
@@ -398,201 +384,6 @@ __device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], in
     for (int i = 0; i < 128; i += kBlockCols)
       store_block(block, v, i, out, p.ldo, row0, col + i, p.m, p.n, p.vec_out != 0);
   }
-}
-
-template <Kind K, Epilogue E, class T>
-__global__ void __launch_bounds__(kThreads, 1)
-    feed_tile_kernel(const __grid_constant__ Maps maps, const Params p) {
-  constexpr int kStageBytes = stage_bytes<K>();
-  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
-  constexpr int kElems = K == Kind::f16 ? 64 : 128; // map elements per 128-byte row
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
-  uint64_t* empty = full + kStages;
-  uint64_t* acc_full = empty + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  // Tiles in groups of 8 row tiles, so a wave of CTAs shares both operands' tiles in L2.
-  const int per_batch = p.tiles_m * p.tiles_n;
-  const int batch = blockIdx.x / per_batch, tile = blockIdx.x % per_batch;
-  const int span = 8 * p.tiles_n, first_m = (tile / span) * 8;
-  const int group_m = min(8, p.tiles_m - first_m);
-  const int m0 = (first_m + (tile % span) % group_m) * 128;
-  const int n0 = ((tile % span) / group_m) * kTileN;
-
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(acc_full, 1);
-    *abort_flag = 0;
-    fence_mbarrier_init();
-  }
-  if (warp == 1)
-    tc::tmem_alloc<1>(tmem_slot, kTmemCols);
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t sbase = smem_u32(smem);
-
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      int issued = 0;
-      for (int kt = 0; kt < p.k_tiles; ++kt) {
-        const int s = kt % kStages, fill = kt / kStages;
-        if (*abort_flag)
-          break;
-        if (fill > 0 && !mbar_wait_bounded(&empty[s], (fill - 1) & 1, p.timeout_ns)) {
-          atomicOr(&feed_error, 2u);
-          *abort_flag = 1;
-          break;
-        }
-        const int seg = kt >= p.k_split;
-        const CUtensorMap* ma = &maps.a[seg | batch];
-        const int k0 = (kt - (seg ? p.k_split : 0)) * kElems;
-        const uint32_t bar = smem_u32(&full[s]);
-        const uint32_t dst = sbase + s * kStageBytes;
-        uint32_t bytes = 3 * kPart;
-        int atoms = 2;
-        if constexpr (K == Kind::mxf4) {
-          atoms = min(2, p.scale_k - 2 * kt);
-          bytes += 3 * 512 * atoms;
-        }
-        mbar_arrive_expect_tx(&full[s], bytes);
-        if (K == Kind::f16 && p.a_mn) {
-          tc::tma_load<1>(dst, ma, bar, m0, k0);
-          tc::tma_load<1>(dst + kPart / 2, ma, bar, m0 + 64, k0);
-        } else {
-          tc::tma_load<1>(dst, ma, bar, k0, m0);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : seg];
-          const int row = E == Epilogue::gated ? n0 : n0 + 128 * j;
-          const uint32_t d = dst + (1 + j) * kPart;
-          if (K == Kind::f16 && p.b_mn) {
-            tc::tma_load<1>(d, mb, bar, row, k0);
-            tc::tma_load<1>(d + kPart / 2, mb, bar, row + 64, k0);
-          } else {
-            tc::tma_load<1>(d, mb, bar, k0, row);
-          }
-        }
-        if constexpr (K == Kind::mxf4) {
-          const uint32_t sc = dst + 3 * kPart;
-          bulk_load(sc, p.scale_a + (static_cast<size_t>(m0 / 128) * p.scale_k + 2 * kt) * 512,
-                    512 * atoms, bar);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // A plain tile's second part may lie past the last row tile: its columns are not
-            // stored, so any scales do.
-            const int rt = E == Epilogue::gated ? n0 / 128 : min(n0 / 128 + j, p.scale_rows_b - 1);
-            bulk_load(sc + 1024 * (1 + j),
-                      p.scale_b[E == Epilogue::gated ? j : 0] +
-                          (static_cast<size_t>(rt) * p.scale_k + 2 * kt) * 512,
-                      512 * atoms, bar);
-          }
-        }
-        ++issued;
-      }
-      // Drain: every stage filled here has been consumed (or times out) before exit.
-      for (int kt = issued > kStages ? issued - kStages : 0; kt < issued; ++kt) {
-        if (!mbar_wait_bounded(&empty[kt % kStages], (kt / kStages) & 1, p.timeout_ns)) {
-          atomicOr(&feed_error, 4u);
-          break;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      for (int kt = 0; kt < p.k_tiles; ++kt) {
-        const int s = kt % kStages;
-        if (*abort_flag)
-          break;
-        if (!mbar_wait_bounded(&full[s], (kt / kStages) & 1, p.timeout_ns)) {
-          atomicOr(&feed_error, 1u);
-          *abort_flag = 1;
-          break;
-        }
-        tc::fence_after();
-        const uint32_t a = sbase + s * kStageBytes, b = a + kPart;
-        if constexpr (K == Kind::f16) {
-          const uint64_t da = p.a_mn ? tc::desc_mnmajor(a) : tc::desc_kmajor(a);
-          const uint64_t db = p.b_mn ? tc::desc_mnmajor(b) : tc::desc_kmajor(b);
-          const uint64_t sa = p.a_mn ? 128 : 2, sb = p.b_mn ? 128 : 2; // 16-byte units per step
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            tc::mma_f16<1>(tmem, da + kk * sa, db + kk * sb, p.idesc, (kt | kk) ? 1u : 0u);
-        } else {
-          const uint32_t sc = a + 3 * kPart;
-          const uint32_t sfa = tmem + kScaleCol + s * kScaleCols, sfb = sfa + 8;
-          const int steps = kt == p.k_tiles - 1 ? p.last_steps : 4;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            if (2 * g < steps) {
-              copy_scales(sfa + 4 * g, sc + 512 * g);
-              copy_scales(sfb + 8 * g, sc + 1024 + 512 * g);
-              copy_scales(sfb + 8 * g + 4, sc + 2048 + 512 * g);
-            }
-          }
-          const uint64_t da = tc::desc_kmajor(a), db = tc::desc_kmajor(b);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t id = (kk & 1) * 2; // byte of the scale column for this step
-            if (kk < steps)
-              mma_mxf4(tmem, da + kk * 2, db + kk * 2, p.idesc | (id << 4) | (id << 29),
-                       sfa + 4 * (kk >> 1), sfb + 8 * (kk >> 1), (kt | kk) ? 1u : 0u);
-          }
-        }
-        tc::mma_commit<1>(smem_u32(&empty[s]));
-      }
-      tc::mma_commit<1>(smem_u32(acc_full));
-    }
-    __syncwarp();
-  } else {
-    // ---------------------------------------------------------------- epilogue
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    const int row = m0 + 32 * quad + lane;
-    const bool ok = mbar_wait_bounded(acc_full, 0, p.timeout_ns * 4);
-    if (!ok) {
-      atomicOr(&feed_error, 8u);
-      *abort_flag = 1;
-    }
-    tc::fence_after();
-    if (__all_sync(0xffffffffu, ok && !*abort_flag)) {
-      const uint32_t t_row = tmem + (static_cast<uint32_t>(32 * quad) << 16);
-      T* out = static_cast<T*>(p.out[batch]) + static_cast<long long>(row) * p.ldo;
-      for (int c0 = half * (kTileN / 2); c0 < (half + 1) * (kTileN / 2); c0 += 16)
-        epilogue_chunk<E, T>(p, t_row, c0, n0 + c0, row, out);
-    }
-    tc::fence_before();
-  }
-
-  __syncthreads();
-  if (warp == 1) {
-    tc::fence_after();
-    tc::tmem_free<1>(tmem, kTmemCols);
-  }
-}
-
-template <Kind K, Epilogue E, class T>
-cudaError_t launch_tiles(const Maps& maps, const Params& p, cudaStream_t stream) {
-  static std::atomic<uint64_t> done{0};
-  const auto kernel = feed_tile_kernel<K, E, T>;
-  if (cudaError_t e = tc::allow_smem(kernel, smem_bytes<K>(), done); e != cudaSuccess)
-    return e;
-  const long long grid = static_cast<long long>(p.batches) * p.tiles_m * p.tiles_n;
-  if (grid <= 0 || grid > 0x7fffffffll)
-    return cudaErrorInvalidConfiguration;
-  kernel<<<static_cast<unsigned>(grid), kThreads, smem_bytes<K>(), stream>>>(maps, p);
-  return cudaGetLastError();
 }
 
 inline cudaError_t read_and_clear_feed_error(unsigned int* out, cudaStream_t stream) {

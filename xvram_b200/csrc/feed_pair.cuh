@@ -1,18 +1,18 @@
-// feed_pair.cuh -- the persistent CTA-pair form of the feed-forward tile kernel (feed_tile.cuh),
-// for 16-bit operands and more than 128 rows.
+// feed_pair.cuh -- the persistent CTA-pair kernel of the feed-forward operators, for more than
+// 128 rows (operands, epilogues and the accumulators' columns: feed_common.cuh).
 //
 // A cluster of two CTAs computes accumulators of 256 rows x 256 columns (tcgen05
-// cta_group::2): each CTA holds 128 rows of A and one 128-row part of B -- the gate's and the up
-// projection's rows of the same features for the gated form, so an output's two
-// pre-activations meet in one TMEM lane.  Two accumulators fill TMEM, used in one of two ways:
+// cta_group::2): each CTA holds 128 rows of A and one of the two 128-row parts of B.
 //
-//   HALVES = 1  a tile is 256 rows; the accumulators alternate, so the epilogue of a tile runs
-//               under the next tile's MMAs;
-//   HALVES = 2  a tile is 512 rows, 256 per CTA, both accumulators over the same B: a quarter
-//               less operand traffic per FLOP.  The epilogue first empties an accumulator into
-//               registers and hands it back, and the next tile's first stages run on accumulator
-//               0 alone (kAhead stages) before accumulator 1 is needed, so the MMAs wait only
-//               for the first emptying.
+//   16-bit, HALVES = 1  a tile is 256 rows; two accumulators fill TMEM and alternate, so the
+//               epilogue of a tile runs under the next tile's MMAs;
+//   16-bit, HALVES = 2  a tile is 512 rows, 256 per CTA, both accumulators over the same B: a
+//               quarter less operand traffic per FLOP.  The epilogue first empties an
+//               accumulator into registers and hands it back, and the next tile's first stages
+//               run on accumulator 0 alone (kAhead stages) before accumulator 1 is needed, so
+//               the MMAs wait only for the first emptying;
+//   MXFP4       a tile is 256 rows with one accumulator, emptied into registers first; the
+//               other TMEM columns hold the stages' scales (each CTA's own A rows, all B rows).
 //
 //   warp 0      one lane per CTA: TMA loads into the stage ring, completion on the leader's
 //               barrier;
@@ -23,20 +23,19 @@
 //               stores are whole 128-byte lines.
 #pragma once
 
-#include "feed_tile.cuh"
+#include "feed_common.cuh"
 
 namespace xvram::feed {
 
-constexpr int kPairStages = 4;
 constexpr int kAhead = 3;
-template <int HALVES>
-__host__ __device__ constexpr uint32_t pair_stage_bytes() {
-  return (HALVES + 1) * kPart;
-}
-template <int HALVES>
-__host__ __device__ constexpr int pair_smem_bytes() {
-  return kPairStages * pair_stage_bytes<HALVES>() + 8 * kStageBlock + 1024 + 256;
-}
+template <Kind K, int HALVES>
+struct PairShape {
+  static constexpr int kStages = K == Kind::mxf4 ? 5 : 4;
+  static constexpr int kSlots = K == Kind::mxf4 ? 1 : 2; // accumulators
+  static constexpr uint32_t kScales = (HALVES + 1) * kPart; // offset of a stage's scales
+  static constexpr uint32_t kStage = kScales + (K == Kind::mxf4 ? kScaleBytes : 0);
+  static constexpr int kSmem = kStages * kStage + 8 * kStageBlock + 1024 + 256;
+};
 
 // The tile's batch and first row and column.  Tiles run in groups of 8 row tiles, so the
 // pairs that work at the same time share both operands' tiles in L2.
@@ -51,11 +50,14 @@ __device__ __forceinline__ void tile_origin(const Params& p, int t, int rows, in
   n0 = ((tile % span) / group_m) * cols;
 }
 
-template <Epilogue E, class T, int HALVES>
+template <Kind K, Epilogue E, class T, int HALVES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     feed_pair_kernel(const __grid_constant__ Maps maps, const Params p) {
   constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
-  constexpr uint32_t kStage = pair_stage_bytes<HALVES>();
+  using Shape = PairShape<K, HALVES>;
+  constexpr int kPairStages = Shape::kStages, kSlots = Shape::kSlots;
+  constexpr uint32_t kStage = Shape::kStage;
+  constexpr int kElems = K == Kind::f16 ? 64 : 128; // map elements per 128-byte row
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -113,25 +115,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const int seg = kt >= p.k_split;
           const CUtensorMap* ma = &maps.a[seg | batch];
           const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? rank : seg];
-          const int k0 = (kt - (seg ? p.k_split : 0)) * 64;
+          const int k0 = (kt - (seg ? p.k_split : 0)) * kElems;
           const uint32_t bar = tc::cluster_addr(smem_u32(&full[s]), 0);
           const uint32_t a = sbase + s * kStage, b = a + HALVES * kPart;
           if (rank == 0)
             mbar_arrive_expect_tx(&full[s], 2 * kStage); // both CTAs' copies
 #pragma unroll
           for (int i = 0; i < HALVES; ++i) {
-            if (p.a_mn) {
+            if (K == Kind::f16 && p.a_mn) {
               tc::tma_load<2>(a + i * kPart, ma, bar, m0 + 128 * i, k0);
               tc::tma_load<2>(a + i * kPart + kPart / 2, ma, bar, m0 + 128 * i + 64, k0);
             } else {
               tc::tma_load<2>(a + i * kPart, ma, bar, k0, m0 + 128 * i);
             }
           }
-          if (p.b_mn) {
+          if (K == Kind::f16 && p.b_mn) {
             tc::tma_load<2>(b, mb, bar, row, k0);
             tc::tma_load<2>(b + kPart / 2, mb, bar, row + 64, k0);
           } else {
             tc::tma_load<2>(b, mb, bar, k0, row);
+          }
+          if constexpr (K == Kind::mxf4) {
+            const uint32_t sc = sbase + s * kStage + Shape::kScales;
+            tc::tma_load<2>(sc, &maps.scale_a, bar, kt * 256, m0 / 128);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              tc::tma_load<2>(sc + kScaleTile * (1 + j),
+                              &maps.scale_b[E == Epilogue::gated ? j : 0], bar, kt * 256,
+                              E == Epilogue::gated ? n0 / 128 : n0 / 128 + j);
           }
           ++issued;
           if (++s == kPairStages) {
@@ -152,7 +163,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------- MMA issuer (pair leader)
     if (rank == 0 && lane == 0) {
       const uint32_t sempty = smem_u32(empty), sacc = smem_u32(acc_full);
-      const uint64_t sa = p.a_mn ? 128 : 2, sb = p.b_mn ? 128 : 2; // 16-byte units per step
       int s = 0;
       uint32_t phase = 0;
       int units = 0; // accumulators used so far
@@ -160,21 +170,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         atomicOr(&feed_error, 1u);
         *abort_flag = 1;
       };
-      const auto take = [&](int unit) { // accumulator unit & 1 is free
-        const int use = unit >> 1;
-        const bool ok =
-            use == 0 || mbar_wait_bounded(&acc_empty[unit & 1], (use - 1) & 1, p.timeout_ns);
+      const auto take = [&](int unit) { // accumulator unit % kSlots is free
+        const int use = unit / kSlots;
+        const bool ok = use == 0 || mbar_wait_bounded(&acc_empty[unit % kSlots], (use - 1) & 1,
+                                                      p.timeout_ns);
         tc::fence_after();
         return ok;
       };
       const auto multiply = [&](int stage, int half, uint32_t d, bool first_k) {
-        const uint32_t a = sbase + stage * kStage + half * kPart;
-        const uint32_t b = sbase + stage * kStage + HALVES * kPart;
-        const uint64_t da = p.a_mn ? tc::desc_mnmajor(a) : tc::desc_kmajor(a);
-        const uint64_t db = p.b_mn ? tc::desc_mnmajor(b) : tc::desc_kmajor(b);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc::mma_f16<2>(d, da + kk * sa, db + kk * sb, p.idesc, (first_k && kk == 0) ? 0u : 1u);
+        const uint32_t base = sbase + stage * kStage;
+        const uint32_t a = base + half * kPart, b = base + HALVES * kPart;
+        if constexpr (K == Kind::f16)
+          stage_f16<2>(p, d, a, b, first_k);
+        else
+          stage_mxf4<2>(p, d, a, b, base + Shape::kScales, tmem + kScaleCol + stage * kScaleCols,
+                        first_k);
       };
       const auto next = [&] {
         if (++s == kPairStages) {
@@ -188,7 +198,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           fail();
           break;
         }
-        const uint32_t d0 = tmem + 256 * (units & 1);
+        const uint32_t d0 = tmem + 256 * (units % kSlots);
         int kt = 0;
         if constexpr (HALVES == 2) {
           // The first stages on accumulator 0 alone, then the same stages on accumulator 1.
@@ -226,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           next();
         }
         if (!stop) {
-          tc::mma_commit_both(sacc + 8 * (units & 1));
+          tc::mma_commit_both(sacc + 8 * (units % kSlots));
           if constexpr (HALVES == 2)
             tc::mma_commit_both(sacc + 8);
         }
@@ -245,9 +255,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tile_origin(p, t, 256 * HALVES, kTileN, batch, m0, n0);
       T* out = static_cast<T*>(p.out[batch]);
       for (int i = 0; i < HALVES; ++i, ++unit) {
-        const int buf = unit & 1;
+        const int buf = unit % kSlots;
         const int row0 = m0 + 128 * (HALVES * static_cast<int>(rank) + i) + 32 * quad;
-        const bool ok = mbar_wait_bounded(&acc_full[buf], (unit >> 1) & 1, p.timeout_ns * 4);
+        const bool ok = mbar_wait_bounded(&acc_full[buf], (unit / kSlots) & 1,
+                                          p.timeout_ns * 4);
         if (!ok) {
           atomicOr(&feed_error, 8u);
           *abort_flag = 1;
@@ -280,11 +291,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-template <Epilogue E, class T, int HALVES>
+template <Kind K, Epilogue E, class T, int HALVES>
 cudaError_t launch_pairs(const Maps& maps, Params p, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  const auto kernel = feed_pair_kernel<E, T, HALVES>;
-  constexpr int smem = pair_smem_bytes<HALVES>();
+  const auto kernel = feed_pair_kernel<K, E, T, HALVES>;
+  constexpr int smem = PairShape<K, HALVES>::kSmem;
+  static_assert(smem <= 232448, "shared memory of one CTA per SM");
   if (cudaError_t e = tc::allow_smem(kernel, smem, done); e != cudaSuccess)
     return e;
   p.tiles_m = (p.m + 256 * HALVES - 1) / (256 * HALVES);

@@ -7,7 +7,7 @@
 // instead of 5 NV).  Bound by reading the weights from HBM; x comes from L1.
 #pragma once
 
-#include "feed_tile.cuh"
+#include "feed_common.cuh"
 
 namespace xvram::feed {
 

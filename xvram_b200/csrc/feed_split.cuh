@@ -1,0 +1,333 @@
+// feed_split.cuh -- the tensor-core kernel of the feed-forward operators for at most 128 rows
+// (operands, epilogues and the accumulator's columns: feed_common.cuh).
+//
+// Bound by reading the weights from HBM: a 128 x 256 accumulator takes all rows of A, so each
+// weight is read once, and M = 128 MMAs on fewer rows still finish inside the time of the
+// loads.  To occupy all SMs when there are few feature tiles, a cluster of p.splits CTAs
+// shares a tile and each takes a range of K; the partial sums meet in distributed shared
+// memory, where each CTA adds up a share of the columns in rank order (the same bits every
+// time) and applies the epilogue.
+//
+// A's stage holds only ceil(m / 8) * 8 rows: the MMA's other rows read whatever follows in
+// shared memory, and those accumulator rows are never looked at.
+//
+//   warp 0      one lane: TMA loads; weights first, A once the preceding kernel (the
+//               quantisation of A, launched with programmatic overlap) is complete;
+//   warp 1      one lane: issues the MMAs;
+//   warps 2..9  empty the accumulator into shared memory; then all warps reduce and finish.
+#pragma once
+
+#include "feed_common.cuh"
+
+#include <algorithm>
+
+namespace xvram::feed {
+
+struct SplitParams {
+  Params p;
+  int splits;      // cluster size
+  int stages;      // ring depth
+  int a_bytes;     // A's bytes per stage
+};
+
+constexpr int kSplitSmem = 222 * 1024;
+constexpr int kSplitRing = kSplitSmem - 2048; // the rest: alignment and barriers
+constexpr int kSplitMaxStages = 12;
+constexpr int kPitch = 256 + 4; // floats per row of the partial sums
+
+__device__ __forceinline__ float4 load_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+template <Kind K, Epilogue E, class T>
+__global__ void __launch_bounds__(kThreads, 1)
+    feed_split_kernel(const __grid_constant__ Maps maps, const SplitParams q) {
+  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
+  constexpr int kElems = K == Kind::f16 ? 64 : 128; // map elements per 128-byte row
+  const Params& p = q.p;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSplitRing);
+  uint64_t* empty = full + kSplitMaxStages;
+  uint64_t* acc_full = empty + kSplitMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int rank = q.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
+  const int n0 = static_cast<int>(blockIdx.x / q.splits) * kTileN;
+  const int k_begin = static_cast<int>(static_cast<long long>(p.k_tiles) * rank / q.splits);
+  const int k_end = static_cast<int>(static_cast<long long>(p.k_tiles) * (rank + 1) / q.splits);
+  const uint32_t b_off = q.a_bytes, scale_off = b_off + 2 * kPart;
+  const uint32_t stage_bytes = scale_off + (K == Kind::mxf4 ? kScaleBytes : 0);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < q.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 1)
+    tc::tmem_alloc<1>(tmem_slot, kTmemCols);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sbase = smem_u32(smem);
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      const auto load_b = [&](int kt, int s) {
+        const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+        const int k0 = kt * kElems;
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : 0];
+          const int row = E == Epilogue::gated ? n0 : n0 + 128 * j;
+          const uint32_t d = base + b_off + j * kPart;
+          if (K == Kind::f16 && p.b_mn) {
+            tc::tma_load<1>(d, mb, bar, row, k0);
+            tc::tma_load<1>(d + kPart / 2, mb, bar, row + 64, k0);
+          } else {
+            tc::tma_load<1>(d, mb, bar, k0, row);
+          }
+          if constexpr (K == Kind::mxf4)
+            tc::tma_load<1>(base + scale_off + kScaleTile * (1 + j),
+                            &maps.scale_b[E == Epilogue::gated ? j : 0], bar, kt * 256,
+                            row / 128);
+        }
+      };
+      const auto load_a = [&](int kt, int s) {
+        const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+        const int k0 = kt * kElems;
+        if (K == Kind::f16 && p.a_mn) {
+          tc::tma_load<1>(base, &maps.a[0], bar, 0, k0);
+          tc::tma_load<1>(base + kPart / 2, &maps.a[0], bar, 64, k0);
+        } else {
+          tc::tma_load<1>(base, &maps.a[0], bar, k0, 0);
+        }
+        if constexpr (K == Kind::mxf4)
+          tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);
+      };
+      const int count = k_end - k_begin, ahead = min(count, q.stages);
+      for (int i = 0; i < ahead; ++i)
+        load_b(k_begin + i, i);
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < ahead; ++i)
+        load_a(k_begin + i, i);
+      int issued = ahead, s = 0;
+      uint32_t phase = 0;
+      for (; issued < count; ++issued) {
+        if (*abort_flag || !mbar_wait_bounded(&empty[s], phase, p.timeout_ns)) {
+          atomicOr(&feed_error, 2u);
+          *abort_flag = 1;
+          break;
+        }
+        load_b(k_begin + issued, s);
+        load_a(k_begin + issued, s);
+        if (++s == q.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+      // Drain: every stage filled here has been consumed (or times out) before exit.
+      for (int i = max(0, issued - q.stages); i < issued; ++i) {
+        if (!mbar_wait_bounded(&empty[i % q.stages], (i / q.stages) & 1, p.timeout_ns)) {
+          atomicOr(&feed_error, 4u);
+          break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 0;
+      for (int kt = k_begin; kt < k_end; ++kt) {
+        if (*abort_flag || !mbar_wait_bounded(&full[s], phase, p.timeout_ns)) {
+          atomicOr(&feed_error, 1u);
+          *abort_flag = 1;
+          break;
+        }
+        tc::fence_after();
+        const uint32_t a = sbase + s * stage_bytes, b = a + b_off;
+        if constexpr (K == Kind::f16)
+          stage_f16<1>(p, tmem, a, b, kt == k_begin);
+        else
+          stage_mxf4<1>(p, tmem, a, b, a + scale_off, tmem + kScaleCol + (s % 10) * kScaleCols,
+                        kt == k_begin);
+        tc::mma_commit<1>(smem_u32(&empty[s]));
+        if (++s == q.stages) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+      tc::mma_commit<1>(smem_u32(acc_full));
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------- accumulator to shared memory
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const bool ok = mbar_wait_bounded(acc_full, 0, p.timeout_ns * 4);
+    if (!ok) {
+      atomicOr(&feed_error, 8u);
+      *abort_flag = 1;
+    }
+    tc::fence_after();
+    if (32 * quad < p.m && __all_sync(0xffffffffu, ok && !*abort_flag)) {
+      const int row = 32 * quad + lane;
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(32 * quad) << 16);
+      float* dst = reinterpret_cast<float*>(smem) + row * kPitch;
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t r[2][16];
+        tc::tmem_ld16(t_row + 128 * half + c, r[0]);
+        tc::tmem_ld16(t_row + 128 * half + c + 16, r[1]);
+        tc::tmem_wait_ld();
+        if (row < p.m) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(dst + 128 * half + c + i) =
+                make_uint4(r[i / 16][i % 16], r[i / 16][i % 16 + 1], r[i / 16][i % 16 + 2],
+                           r[i / 16][i % 16 + 3]);
+        }
+        __syncwarp();
+      }
+    }
+    tc::fence_before();
+  }
+
+  // Every wait above is bounded, so all warps of all the cluster's CTAs come here.
+  __syncthreads();
+  if (q.splits > 1)
+    tc::cluster_sync();
+  if (warp == 1) {
+    tc::fence_after();
+    tc::tmem_free<1>(tmem, kTmemCols);
+  }
+  // ---------------------------------------------------------- reduce and finish
+  const int cols = kTileN / q.splits; // a multiple of 16
+  const int groups = cols / 4;
+  T* out = static_cast<T*>(p.out[0]);
+  for (int i = tid; i < p.m * groups; i += kThreads) {
+    const int r = i / groups, c = rank * cols + (i - r * groups) * 4;
+    const int col = n0 + c;
+    if (col >= p.n)
+      continue;
+    float v[4] = {}, w[4] = {};
+    for (int s = 0; s < q.splits; ++s) {
+      const uint32_t local = sbase + (r * kPitch + c) * 4;
+      const uint32_t from = q.splits > 1 ? tc::cluster_addr(local, s) : local;
+      const float4 x = load_cluster(from);
+      v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+      if constexpr (E == Epilogue::gated) {
+        const float4 y = load_cluster(from + 128 * 4);
+        w[0] += y.x, w[1] += y.y, w[2] += y.z, w[3] += y.w;
+      }
+    }
+    add_bias<T>(p.bias0, col, p.n, v);
+    if constexpr (E == Epilogue::gated) {
+      add_bias<T>(p.bias1, col, p.n, w);
+      if (p.save_gate) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < p.n) {
+            p.save_gate[r * p.lds + col + j] = v[j];
+            p.save_up[r * p.lds + col + j] = w[j];
+          }
+      }
+      gate<sizeof(T) == 2>(p.act, v, w);
+    } else if (p.relu) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] = act_of<kRelu, true>(v[j]);
+    }
+    T* dst = out + r * p.ldo + col;
+    if (p.vec_out && col + 4 <= p.n) {
+      alignas(16) T t[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        t[j] = from_float<T>(v[j]);
+      if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t);
+      else
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < p.n)
+          dst[j] = from_float<T>(v[j]);
+    }
+  }
+  if (q.splits > 1)
+    tc::cluster_sync(); // no CTA leaves while another reads its sums
+}
+
+// Rows of A that a stage holds.
+inline int split_rows(int m) { return std::min(128, (m + 7) / 8 * 8); }
+
+// `after`: launched behind a kernel of the same stream that allows programmatic overlap.
+template <Kind K, Epilogue E, class T>
+cudaError_t launch_split(const Maps& maps, const Params& p, bool after, cudaStream_t stream) {
+  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
+  static std::atomic<uint64_t> done{0};
+  const auto kernel = feed_split_kernel<K, E, T>;
+  if (cudaError_t e = tc::allow_smem(kernel, kSplitSmem, done); e != cudaSuccess)
+    return e;
+  SplitParams q;
+  q.p = p;
+  q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
+  const int stage = q.a_bytes + 2 * kPart + (K == Kind::mxf4 ? kScaleBytes : 0);
+  q.stages = std::min(K == Kind::mxf4 ? 10 : kSplitMaxStages, kSplitRing / stage);
+  // A stage of all SMs takes about 0.75 us of HBM time; joining costs about 1 us and a little
+  // per CTA.  The split with the least of waves x stages, and joins, wins.
+  const long long tiles = (p.n + kTileN - 1) / kTileN, sms = tc::sm_count();
+  double best = 0;
+  q.splits = 1;
+  for (int s = 1; s <= 8 && s <= p.k_tiles; s *= 2) {
+    const double t = 0.75 * static_cast<double>((tiles * s + sms - 1) / sms) *
+                         ((p.k_tiles + s - 1) / s) +
+                     (s > 1 ? 1.0 + 0.1 * s : 0.0);
+    if (s == 1 || t < best) {
+      best = t;
+      q.splits = s;
+    }
+  }
+  const long long grid = tiles * q.splits;
+  if (grid > 0x7fffffffll)
+    return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(grid));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = kSplitSmem;
+  config.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  unsigned n = 0;
+  if (q.splits > 1) {
+    attrs[n].id = cudaLaunchAttributeClusterDimension;
+    attrs[n].val.clusterDim.x = q.splits;
+    attrs[n].val.clusterDim.y = attrs[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (after) {
+    attrs[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  config.attrs = attrs;
+  config.numAttrs = n;
+  return cudaLaunchKernelEx(&config, kernel, maps, q);
+}
+
+} // namespace xvram::feed

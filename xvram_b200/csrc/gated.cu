@@ -17,7 +17,7 @@
 // stay separate kernels.
 #include "feed_pair.cuh"
 #include "feed_rows.cuh"
-#include "feed_tile.cuh"
+#include "feed_split.cuh"
 #include "kernels.hpp"
 
 #include <algorithm>
@@ -216,10 +216,10 @@ cudaError_t launch_bias_sum(const float* partial, int m, int h, void* dbg, void*
 // Map of an operand with `rows` rows (the output's axis) and `k` values each: K-major
 // ([rows][ld]) or M-/N-major ([k][ld]).
 bool operand_map(CUtensorMap* map, bool bf16, const void* base, long long rows, long long k,
-                 long long ld, bool mn) {
+                 long long ld, bool mn, uint32_t box_rows = 128) {
   const auto type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   return mn ? tc::encode_map(map, type, base, rows, k, ld * 2, 64, 64)
-            : tc::encode_map(map, type, base, k, rows, ld * 2, 64, 128);
+            : tc::encode_map(map, type, base, k, rows, ld * 2, 64, box_rows);
 }
 
 Params base_params(bool bf16, int m, int n, int k_tiles, bool a_mn, bool b_mn, int tile_n) {
@@ -227,36 +227,34 @@ Params base_params(bool bf16, int m, int n, int k_tiles, bool a_mn, bool b_mn, i
   p.m = m;
   p.n = n;
   p.k_tiles = p.k_split = k_tiles;
-  p.tiles_m = (m + 127) / 128;
   p.tiles_n = (n + tile_n - 1) / tile_n;
   p.batches = 1;
   p.a_mn = a_mn;
   p.b_mn = b_mn;
-  p.idesc = idesc_f16(bf16, a_mn, b_mn, 128, 256);
+  p.idesc = idesc_f16(bf16, a_mn, b_mn, 256, 256);
   p.timeout_ns = kernel_wait_limit_ns();
   return p;
 }
 
-// The pair kernel above one row tile, with 512-row tiles where their waves cost less: one runs in
-// 1.85 times a 256-row tile's time (8192 x 4096 x 8192, seconds of it back to back under the
-// power cap: 832 us against 859; 2048 rows, 4 waves against 7: 231 against 222).
+// The pair kernel, with 512-row tiles where their waves cost less: one runs in 1.85 times a
+// 256-row tile's time (8192 x 4096 x 8192, seconds of it back to back under the power cap: 832 us
+// against 859; 2048 rows, 4 waves against 7: 231 against 222).
 template <Epilogue E, class T>
-cudaError_t launch_16(const Maps& maps, Params p, bool bf16, cudaStream_t stream) {
-  if (p.m <= 128)
-    return launch_tiles<Kind::f16, E, T>(maps, p, stream);
-  p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 256, 256);
+cudaError_t launch_16(const Maps& maps, const Params& p, cudaStream_t stream) {
   const long long pairs = tc::sm_count() / 2, cols = static_cast<long long>(p.batches) * p.tiles_n;
   const long long one = (cols * ((p.m + 255) / 256) + pairs - 1) / pairs;
   const long long two = (cols * ((p.m + 511) / 512) + pairs - 1) / pairs;
-  return 1.85 * two < one ? launch_pairs<E, T, 2>(maps, p, stream)
-                          : launch_pairs<E, T, 1>(maps, p, stream);
+  return 1.85 * two < one ? launch_pairs<Kind::f16, E, T, 2>(maps, p, stream)
+                          : launch_pairs<Kind::f16, E, T, 1>(maps, p, stream);
 }
 
 template <class T>
 cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStream_t stream) {
   constexpr bool bf16 = std::is_same_v<T, __nv_bfloat16>;
   Maps maps;
-  if (!operand_map(&maps.a[0], bf16, q.x, q.m, q.k, q.ldx, q.x_transposed) ||
+  const bool split = q.m <= 128;
+  if (!operand_map(&maps.a[0], bf16, q.x, q.m, q.k, q.ldx, q.x_transposed,
+                   split ? split_rows(q.m) : 128) ||
       !operand_map(&maps.b[0], bf16, q.w_gate, q.h, q.k, q.ld_gate, q.w_transposed) ||
       !operand_map(&maps.b[1], bf16, q.w_up, q.h, q.k, q.ld_up, q.w_transposed))
     return cudaErrorInvalidValue;
@@ -271,7 +269,11 @@ cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStre
   p.save_gate = q.pre_gate;
   p.save_up = q.pre_up;
   p.lds = q.ld_pre;
-  return launch_16<Epilogue::gated, T>(maps, p, bf16, stream);
+  if (split) {
+    p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 128, 256);
+    return launch_split<Kind::f16, Epilogue::gated, T>(maps, p, false, stream);
+  }
+  return launch_16<Epilogue::gated, T>(maps, p, stream);
 }
 
 template <class T>
@@ -305,7 +307,7 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[0] = p.out[1] = d.dx;
     p.ldo = d.lddx;
     p.vec_out = d.lddx % 8 == 0 && aligned16(d.dx);
-    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, bf16, stream);
+    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, stream);
         e != cudaSuccess)
       return e;
   }
@@ -325,7 +327,7 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[1] = d.dw_up;
     p.ldo = d.ld_dw;
     p.vec_out = d.ld_dw % 8 == 0 && aligned16(p.out[0]) && aligned16(p.out[1]);
-    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, bf16, stream);
+    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, stream);
         e != cudaSuccess)
       return e;
   }

@@ -141,11 +141,14 @@ cudaError_t read_and_clear_kernel_error_gated(unsigned int* out, cudaStream_t st
 // ceil(cols / 128) tiles of 512 bytes, both 16-byte aligned.  Sizes are positive; lds and ldd in
 // elements of `type`.
 struct Mxfp4Operand {
-  const unsigned char *codes = nullptr, *scales = nullptr;
+  unsigned char *codes = nullptr, *scales = nullptr;
 };
 // out = a b[0]^T (+ bias[0], ReLU), or with b[1] act(a b[0]^T + bias[0]) * (a b[1]^T + bias[1]);
-// out and the biases are of `type`.
+// out and the biases are of `type`.  With x set, x is quantised into a first.
 struct Mxfp4Product {
+  GatedType x_type = GatedType::f32;
+  const void* x = nullptr;
+  long long ldx = 0;
   GatedType type = GatedType::f32;
   int m = 0, n = 0, k = 0, act = 0;
   bool relu = false;

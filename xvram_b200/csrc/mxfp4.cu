@@ -12,7 +12,8 @@
 //   (r % 32) * 16 + (r / 32 % 4) * 4 + b % 4 -- the order in which the tensor core reads them,
 //   so a stage's scales arrive by one bulk copy.  Codes past the last column are 0, scales of
 //   rows and blocks past the end 127 (1.0), so that padding multiplies to zero.
-#include "feed_tile.cuh"
+#include "feed_pair.cuh"
+#include "feed_split.cuh"
 #include "kernels.hpp"
 
 #include <algorithm>
@@ -76,12 +77,14 @@ __device__ __forceinline__ size_t scale_index(long long r, int b, int block_tile
 }
 
 // Four lanes to a block, eight values each.  HBM-bound: the values in, 17 bytes out per block.
-// The grid covers the scales' padded rows and blocks, whose bytes it sets to 127.
+// The grid covers the scales' padded rows and blocks, whose bytes it sets to 127.  A product
+// launched behind it with programmatic overlap may start loading its weights at once.
 template <class T>
 __global__ void __launch_bounds__(256)
     mxfp4_quantize_kernel(const T* __restrict__ src, long long lds, bool vec, int rows, int cols,
                           int blocks, int block_tiles, unsigned char* __restrict__ codes,
                           unsigned char* __restrict__ scales, long long units) {
+  asm volatile("griddepcontrol.launch_dependents;");
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < units; i += gridDim.x * 256ll) {
     const int sub = static_cast<int>(i & 3);
     const long long r = (i >> 2) / (4 * block_tiles);
@@ -171,46 +174,46 @@ cudaError_t dequantize(const unsigned char* codes, const unsigned char* scales, 
   return cudaGetLastError();
 }
 
-bool codes_map(CUtensorMap* map, const void* codes, int rows, int blocks) {
+bool operand_maps(CUtensorMap* codes, CUtensorMap* scales, const Mxfp4Operand& o, int rows,
+                  int blocks, uint32_t box_rows) {
   const uint64_t pitch = static_cast<uint64_t>(blocks) * 16;
-  return tc::encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, pitch, rows, pitch, 128, 128);
+  const uint64_t tiles = (static_cast<uint64_t>(blocks) + 3) / 4;
+  return tc::encode_map(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, o.codes, pitch, rows, pitch, 128,
+                        box_rows) &&
+         tc::encode_map(scales, CU_TENSOR_MAP_DATA_TYPE_UINT32, o.scales, tiles * 128,
+                        (static_cast<uint64_t>(rows) + 127) / 128, tiles * 512, 256, 1, false);
 }
 
 template <Epilogue E, class T>
-cudaError_t product(const Mxfp4Product& q, cudaStream_t stream) {
-  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
+cudaError_t product(const Mxfp4Product& q, bool after, cudaStream_t stream) {
+  constexpr bool gated = E == Epilogue::gated;
+  constexpr int kTileN = gated ? 128 : 256;
   const int blocks = (q.k + kBlock - 1) / kBlock;
+  const bool split = q.m <= 128;
   Maps maps;
-  const bool gated = E == Epilogue::gated;
-  if (!codes_map(&maps.a[0], q.a.codes, q.m, blocks) ||
-      !codes_map(&maps.b[0], q.b[0].codes, q.n, blocks) ||
-      !codes_map(&maps.b[1], q.b[gated ? 1 : 0].codes, q.n, blocks) ||
-      !aligned16(q.a.scales) || !aligned16(q.b[0].scales) || !aligned16(q.b[1].scales))
+  if (!operand_maps(&maps.a[0], &maps.scale_a, q.a, q.m, blocks, split ? split_rows(q.m) : 128))
     return cudaErrorInvalidValue;
+  for (int i = 0; i < 2; ++i)
+    if (!operand_maps(&maps.b[i], &maps.scale_b[i], q.b[gated ? i : 0], q.n, blocks, 128))
+      return cudaErrorInvalidValue;
   maps.a[1] = maps.a[0];
   Params p{};
   p.m = q.m;
   p.n = q.n;
   p.k_tiles = p.k_split = (blocks + 7) / 8;
-  p.last_steps = (blocks - (p.k_tiles - 1) * 8 + 1) / 2;
-  p.tiles_m = (q.m + 127) / 128;
   p.tiles_n = (q.n + kTileN - 1) / kTileN;
   p.batches = 1;
-  p.idesc = idesc_mxf4(128, 256);
   p.act = q.act;
   p.relu = q.relu;
-  p.scale_a = q.a.scales;
-  p.scale_b[0] = q.b[0].scales;
-  p.scale_b[1] = q.b[gated ? 1 : 0].scales;
-  p.scale_k = (blocks + 3) / 4;
-  p.scale_rows_b = (q.n + 127) / 128;
   p.bias0 = q.bias[0];
   p.bias1 = q.bias[1];
   p.out[0] = p.out[1] = q.out;
   p.ldo = q.ldo;
   p.vec_out = vec_rows<T>(q.out, q.ldo);
   p.timeout_ns = kernel_wait_limit_ns();
-  return launch_tiles<Kind::mxf4, E, T>(maps, p, stream);
+  p.idesc = idesc_mxf4(split ? 128 : 256, 256);
+  return split ? launch_split<Kind::mxf4, E, T>(maps, p, after, stream)
+               : launch_pairs<Kind::mxf4, E, T, 1>(maps, p, stream);
 }
 
 } // namespace
@@ -236,17 +239,22 @@ cudaError_t mxfp4_dequantize(GatedType type, const unsigned char* codes,
 }
 
 cudaError_t mxfp4_product(const Mxfp4Product& q, cudaStream_t stream) {
+  const bool after = q.x != nullptr;
+  if (after)
+    if (cudaError_t e = mxfp4_quantize(q.x_type, q.x, q.ldx, q.m, q.k, q.a.codes, q.a.scales, stream);
+        e != cudaSuccess)
+      return e;
   if (q.b[1].codes) {
     switch (q.type) {
-    case GatedType::f16: return product<Epilogue::gated, __half>(q, stream);
-    case GatedType::bf16: return product<Epilogue::gated, __nv_bfloat16>(q, stream);
-    default: return product<Epilogue::gated, float>(q, stream);
+    case GatedType::f16: return product<Epilogue::gated, __half>(q, after, stream);
+    case GatedType::bf16: return product<Epilogue::gated, __nv_bfloat16>(q, after, stream);
+    default: return product<Epilogue::gated, float>(q, after, stream);
     }
   }
   switch (q.type) {
-  case GatedType::f16: return product<Epilogue::plain, __half>(q, stream);
-  case GatedType::bf16: return product<Epilogue::plain, __nv_bfloat16>(q, stream);
-  default: return product<Epilogue::plain, float>(q, stream);
+  case GatedType::f16: return product<Epilogue::plain, __half>(q, after, stream);
+  case GatedType::bf16: return product<Epilogue::plain, __nv_bfloat16>(q, after, stream);
+  default: return product<Epilogue::plain, float>(q, after, stream);
   }
 }
 

@@ -161,6 +161,39 @@ bool mxfp4_operand(uint64_t codes, uint64_t scales) {
   return codes && scales && codes % 16 == 0 && scales % 16 == 0;
 }
 
+xvram_status run_mxfp4(const xvram_b200_mxfp4_product_v1& d, bool gated) {
+  const uint32_t last = gated ? XVRAM_B200_GATE_SIGMOID : XVRAM_B200_ACTIVATION_RELU;
+  if (d.struct_size < sizeof(d) || d.out_type > XVRAM_DATA_FP32 || d.x_type > XVRAM_DATA_FP32 ||
+      d.activation > last || !mxfp4_size(d.m, d.k) || !mxfp4_size(d.n, d.k) || d.k < 1)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  if (d.m == 0 || d.n == 0)
+    return XVRAM_STATUS_SUCCESS;
+  if (!mxfp4_operand(d.x_codes, d.x_scales) || !d.out || d.ld_out < d.n ||
+      !element_aligned(d.out, d.out_type) ||
+      (d.x && (d.ldx < d.k || !element_aligned(d.x, d.x_type))))
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  Mxfp4Product q;
+  for (int i = 0; i < (gated ? 2 : 1); ++i) {
+    if (!mxfp4_operand(d.w_codes[i], d.w_scales[i]) || !element_aligned(d.bias[i], d.out_type))
+      return XVRAM_STATUS_INVALID_ARGUMENT;
+    q.b[i] = {bytes(d.w_codes[i]), bytes(d.w_scales[i])};
+    q.bias[i] = pointer(d.bias[i]);
+  }
+  q.x_type = static_cast<GatedType>(d.x_type);
+  q.x = pointer(d.x);
+  q.ldx = d.ldx;
+  q.type = static_cast<GatedType>(d.out_type);
+  q.m = static_cast<int>(d.m);
+  q.n = static_cast<int>(d.n);
+  q.k = static_cast<int>(d.k);
+  q.act = static_cast<int>(d.activation);
+  q.relu = !gated && d.activation == XVRAM_B200_ACTIVATION_RELU;
+  q.a = {bytes(d.x_codes), bytes(d.x_scales)};
+  q.out = pointer(d.out);
+  q.ldo = d.ld_out;
+  return from_cuda(mxfp4_product(q, as_stream(d.stream)));
+}
+
 } // namespace
 
 extern "C" {
@@ -583,61 +616,14 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
                                     ldd, as_stream(stream)));
 }
 
-XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_linear(
-    uint32_t out_type, int64_t m, int64_t n, int64_t k, uint64_t x_codes, uint64_t x_scales,
-    uint64_t w_codes, uint64_t w_scales, uint64_t bias, uint32_t activation, uint64_t out,
-    int64_t ld_out, uint64_t stream) {
-  if (out_type > XVRAM_DATA_FP32 || activation > XVRAM_B200_ACTIVATION_RELU || !mxfp4_size(m, k) ||
-      !mxfp4_size(n, k) || k < 1)
-    return XVRAM_STATUS_INVALID_ARGUMENT;
-  if (m == 0 || n == 0)
-    return XVRAM_STATUS_SUCCESS;
-  if (!mxfp4_operand(x_codes, x_scales) || !mxfp4_operand(w_codes, w_scales) || !out ||
-      ld_out < n || !element_aligned(out, out_type) || !element_aligned(bias, out_type))
-    return XVRAM_STATUS_INVALID_ARGUMENT;
-  Mxfp4Product q;
-  q.type = static_cast<GatedType>(out_type);
-  q.m = static_cast<int>(m);
-  q.n = static_cast<int>(n);
-  q.k = static_cast<int>(k);
-  q.relu = activation == XVRAM_B200_ACTIVATION_RELU;
-  q.a = {bytes(x_codes), bytes(x_scales)};
-  q.b[0] = {bytes(w_codes), bytes(w_scales)};
-  q.bias[0] = pointer(bias);
-  q.out = pointer(out);
-  q.ldo = ld_out;
-  return from_cuda(mxfp4_product(q, as_stream(stream)));
+XVRAM_B200_API xvram_status XVRAM_CALL
+xvram_b200_mxfp4_linear(const xvram_b200_mxfp4_product_v1* product) {
+  return product ? run_mxfp4(*product, false) : XVRAM_STATUS_INVALID_ARGUMENT;
 }
 
-XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_gated(
-    uint32_t out_type, uint32_t activation, int64_t m, int64_t h, int64_t k, uint64_t x_codes,
-    uint64_t x_scales, uint64_t gate_codes, uint64_t gate_scales, uint64_t up_codes,
-    uint64_t up_scales, uint64_t bias_gate, uint64_t bias_up, uint64_t out, int64_t ld_out,
-    uint64_t stream) {
-  if (out_type > XVRAM_DATA_FP32 || activation > XVRAM_B200_GATE_SIGMOID || !mxfp4_size(m, k) ||
-      !mxfp4_size(h, k) || k < 1)
-    return XVRAM_STATUS_INVALID_ARGUMENT;
-  if (m == 0 || h == 0)
-    return XVRAM_STATUS_SUCCESS;
-  if (!mxfp4_operand(x_codes, x_scales) || !mxfp4_operand(gate_codes, gate_scales) ||
-      !mxfp4_operand(up_codes, up_scales) || !out || ld_out < h ||
-      !element_aligned(out, out_type) || !element_aligned(bias_gate, out_type) ||
-      !element_aligned(bias_up, out_type))
-    return XVRAM_STATUS_INVALID_ARGUMENT;
-  Mxfp4Product q;
-  q.type = static_cast<GatedType>(out_type);
-  q.m = static_cast<int>(m);
-  q.n = static_cast<int>(h);
-  q.k = static_cast<int>(k);
-  q.act = static_cast<int>(activation);
-  q.a = {bytes(x_codes), bytes(x_scales)};
-  q.b[0] = {bytes(gate_codes), bytes(gate_scales)};
-  q.b[1] = {bytes(up_codes), bytes(up_scales)};
-  q.bias[0] = pointer(bias_gate);
-  q.bias[1] = pointer(bias_up);
-  q.out = pointer(out);
-  q.ldo = ld_out;
-  return from_cuda(mxfp4_product(q, as_stream(stream)));
+XVRAM_B200_API xvram_status XVRAM_CALL
+xvram_b200_mxfp4_gated(const xvram_b200_mxfp4_product_v1* product) {
+  return product ? run_mxfp4(*product, true) : XVRAM_STATUS_INVALID_ARGUMENT;
 }
 
 } // extern "C"

@@ -170,11 +170,11 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
 }
 
 // Map of a 2D array of `outer` rows of `inner` elements, `pitch` bytes apart, read in boxes
-// of box_inner (128 bytes, swizzled) x box_outer; false when the base or pitch is not a
+// of box_inner (128 bytes when swizzled) x box_outer; false when the base or pitch is not a
 // multiple of 16 bytes.
 inline bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base,
                        uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner,
-                       uint32_t box_outer) {
+                       uint32_t box_outer, bool swizzle = true) {
   const auto encode = tensor_map_encoder();
   if (!encode || (reinterpret_cast<uintptr_t>(base) & 15u) || (pitch & 15u))
     return false;
@@ -183,7 +183,8 @@ inline bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* b
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t es[2] = {1, 1};
   return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, es,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

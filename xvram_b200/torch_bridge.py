@@ -34,8 +34,9 @@ tensors:
 """
 from __future__ import annotations
 
-import ctypes
 import atexit
+import contextlib
+import ctypes
 import threading
 
 import dataclasses
@@ -44,7 +45,7 @@ import torch
 
 from . import device as xd
 from . import sdk
-from ._native import Gated, lib
+from ._native import Gated, Mxfp4Product, lib
 
 _TF32X3 = 3
 _TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32: sdk.FP32,
@@ -135,6 +136,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 
 # ---------------------------------------------------------------- feed-forward operators
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+_HERE = contextlib.nullcontext()
 _FEED_TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32: sdk.FP32}
 
 
@@ -144,46 +146,47 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _on_device(device: torch.device):
-    """Makes `device` current for the library's calls, which use the current device."""
-    return torch.cuda.device(device)
+def _on_device(index: int):
+    """Makes device `index` current for the library's calls, which use the current device."""
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The stream handle itself: building torch's Stream object costs 2 us of a call of 10.
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(
+    torch._C, "_cuda_getCurrentRawStream") else (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _aligned(x: torch.Tensor, ld: int) -> bool:
-    """Whether the tensor-core kernels can read x in place (float32 needs no alignment)."""
-    return x.dtype == torch.float32 or (x.data_ptr() % 16 == 0 and ld % 8 == 0)
-
-
-def _operand(x: torch.Tensor):
+def _operand(x: torch.Tensor, aligned: bool):
     """(tensor, leading dimension, transposed): x itself where the kernels can read it, else a
-    copy whose rows are padded to 16 bytes."""
+    copy whose rows are padded to 16 bytes.  `aligned`: rows must be multiples of 16 bytes."""
     r, c = x.shape
     s0, s1 = x.stride()
+    per = 16 // x.element_size()
     if r == 1 and s1 == 1:  # one row's stride is never used
-        s0 = (c + 7) // 8 * 8
-    if s1 == 1 and s0 >= c and _aligned(x, s0):
-        return x, s0, 0
-    if s0 == 1 and s1 >= r and _aligned(x, s1):
-        return x, s1, 1
-    ld = (c + 7) // 8 * 8
+        s0 = (c + per - 1) // per * per
+    if not aligned or x.data_ptr() % 16 == 0:
+        if s1 == 1 and s0 >= c and not (aligned and s0 % per):
+            return x, s0, 0
+        if s0 == 1 and s1 >= r and not (aligned and s1 % per):
+            return x, s1, 1
+    ld = (c + per - 1) // per * per
     y = torch.empty((r, ld), dtype=x.dtype, device=x.device)[:, :c]
     y.copy_(x)
     return y, ld, 0
 
 
-def _check_bias(b, h: int, like: torch.Tensor, name: str):
-    if b is None:
-        return None
-    if b.dtype != like.dtype or b.device != like.device or b.dim() != 1 or b.numel() != h:
-        raise ValueError(f"{name} must hold {h} values of the input's type on its device")
+_GATED_SIZE = ctypes.sizeof(Gated)
+_PRODUCT_SIZE = ctypes.sizeof(Mxfp4Product)
+
+
+def _check_bias(b: torch.Tensor, h: int, dtype: torch.dtype, device: torch.device, name: str):
+    if b.dtype != dtype or b.device != device or b.dim() != 1 or b.numel() != h:
+        raise ValueError(f"{name} must hold {h} values of the result's type on its device")
     return b.contiguous()
 
 
@@ -215,20 +218,24 @@ class GatedSaved:
     activation: str
 
 
-def _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act: int):
+def _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act: int, backward: bool):
     """The call's descriptor and the tensors it points to, which must outlive the call."""
-    xo, ldx, xt = _operand(x)
-    go, ldg, gt = _operand(w_gate)
-    uo, ldu, ut = _operand(w_up)
+    (m, k), h = x.shape, w_gate.shape[0]
+    # The float32 GEMM reads any operand, but unaligned ones several times slower than it takes to
+    # copy them; the few-rows kernel reads them at full speed.
+    aligned = x.dtype != torch.float32 or backward or m > 32
+    xo, ldx, xt = _operand(x, aligned)
+    go, ldg, gt = _operand(w_gate, aligned)
+    uo, ldu, ut = _operand(w_up, aligned)
     if gt != ut:  # one weight row-major, the other transposed: bring the latter to rows
         if gt:
-            go, ldg, gt = _operand(w_gate.contiguous())
+            go, ldg, gt = _operand(w_gate.contiguous(), aligned)
         else:
-            uo, ldu, ut = _operand(w_up.contiguous())
-    d = Gated(ctypes.sizeof(Gated), _FEED_TYPES[x.dtype], act, xt, gt, 0, x.shape[0],
-              w_gate.shape[0], x.shape[1], xo.data_ptr(), go.data_ptr(), uo.data_ptr(), ldx, ldg,
-              ldu, _ptr(bias_gate), _ptr(bias_up), _ptr(pre_gate), _ptr(pre_up),
-              0 if pre_gate is None else pre_gate.stride(0), 0, 0, 0)
+            uo, ldu, ut = _operand(w_up.contiguous(), aligned)
+    d = Gated(_GATED_SIZE, _FEED_TYPES[x.dtype], act, xt, gt, 0, m, h, k, xo.data_ptr(),
+              go.data_ptr(), uo.data_ptr(), ldx, ldg, ldu, _ptr(bias_gate), _ptr(bias_up),
+              _ptr(pre_gate), _ptr(pre_up), 0 if pre_gate is None else pre_gate.stride(0), 0, 0,
+              _stream(x.device.index))
     return d, (xo, go, uo)
 
 
@@ -246,21 +253,24 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
     act = _activation(activation)
     _check_gated(x, w_gate, w_up)
     m, h = x.shape[0], w_gate.shape[0]
-    bias_gate = _check_bias(bias_gate, h, x, "bias_gate")
-    bias_up = _check_bias(bias_up, h, x, "bias_up")
-    with _on_device(x.device):
-        out = torch.empty((m, h), dtype=x.dtype, device=x.device)
+    if bias_gate is not None:
+        bias_gate = _check_bias(bias_gate, h, x.dtype, x.device, "bias_gate")
+    if bias_up is not None:
+        bias_up = _check_bias(bias_up, h, x.dtype, x.device, "bias_up")
+    with _on_device(x.device.index):
+        out = x.new_empty((m, h))
         pre_gate = pre_up = None
         if keep:
-            pre = torch.empty((2, m, (h + 3) // 4 * 4), dtype=torch.float32, device=x.device)
-            pre_gate, pre_up = pre[0], pre[1]
-        d, operands = _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act)
-        ws = _gated_workspace(d, 0, x.device)  # noqa: F841  (alive until the launch)
-        d.stream = _stream(x.device)
+            pre_gate, pre_up = torch.empty((2, m, (h + 3) // 4 * 4), dtype=torch.float32,
+                                           device=x.device).unbind()
+        d, operands = _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act,
+                                  False)
+        ws = None
+        if x.dtype == torch.float32:
+            ws = _gated_workspace(d, 0, x.device)  # noqa: F841  (alive until the launch)
         _check(lib.xvram_b200_gated_forward(ctypes.byref(d), out.data_ptr(), h),
                "xvram_b200_gated_forward")
-    saved = GatedSaved(*operands, pre_gate, pre_up, activation) if keep else None
-    return out, saved
+    return out, (GatedSaved(*operands, pre_gate, pre_up, activation) if keep else None)
 
 
 def gated_linear_forward(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu"):
@@ -279,16 +289,15 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     (m, k), h = x.shape, w_gate.shape[0]
     if dh.shape != (m, h) or dh.dtype != x.dtype or dh.device != x.device:
         raise ValueError(f"dh must be a ({m}, {h}) {x.dtype} tensor on {x.device}")
-    with torch.no_grad(), _on_device(x.device):
+    with torch.no_grad(), _on_device(x.device.index):
         if dh.stride(1) != 1 or dh.stride(0) < h:
             dh = dh.contiguous()
         shapes = ((m, k), (h, k), (h, k), (h,), (h,))
         grads = [torch.empty(s, dtype=x.dtype, device=x.device) if n else None
                  for s, n in zip(shapes, needs)]
         d, operands = _gated_desc(x, w_gate, w_up, None, None, saved.pre_gate, saved.pre_up,
-                                  _activation(saved.activation))
+                                  _activation(saved.activation), True)
         ws = _gated_workspace(d, 1, x.device)  # noqa: F841
-        d.stream = _stream(x.device)
         dx, dwg, dwu, dbg, dbu = (_ptr(g) for g in grads)
         _check(lib.xvram_b200_gated_backward(ctypes.byref(d), dh.data_ptr(), max(dh.stride(0), h),
                                              dx, k, dwg, dwu, k, dbg, dbu),
@@ -355,6 +364,16 @@ class Mxfp4Matrix:
         return self.codes.device
 
 
+def _rows(x: torch.Tensor):
+    """(x with contiguous rows, its leading dimension)"""
+    s0, s1 = x.stride()
+    cols = x.shape[1]
+    if s1 != 1 or s0 < cols:
+        x = x.contiguous()
+        s0 = cols
+    return x, s0
+
+
 def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
     """x (rows, cols; float16, bfloat16 or float32, CUDA) in MXFP4: blocks of 32 along each row
     share the scale 2^(floor(log2 max|v|) - 2); elements are rounded to the nearest E2M1 value,
@@ -368,15 +387,13 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("quantize_mxfp4 has no gradient: detach its input")
     rows, cols = x.shape
-    with _on_device(x.device):
-        if x.stride(1) != 1 or x.stride(0) < cols:
-            x = x.contiguous()
-        codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(((rows + 127) // 128, (cols + 127) // 128, 512), dtype=torch.uint8,
-                             device=x.device)
-        _check(lib.xvram_b200_mxfp4_quantize(_FEED_TYPES[x.dtype], rows, cols, x.data_ptr(),
-                                             max(x.stride(0), cols), codes.data_ptr(),
-                                             scales.data_ptr(), _stream(x.device)),
+    with _on_device(x.device.index):
+        x, ldx = _rows(x)
+        codes = x.new_empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8)
+        scales = x.new_empty(((rows + 127) // 128, (cols + 127) // 128, 512), dtype=torch.uint8)
+        _check(lib.xvram_b200_mxfp4_quantize(_FEED_TYPES[x.dtype], rows, cols, x.data_ptr(), ldx,
+                                             codes.data_ptr(), scales.data_ptr(),
+                                             _stream(x.device.index)),
                "xvram_b200_mxfp4_quantize")
     return Mxfp4Matrix(codes, scales, (rows, cols))
 
@@ -389,28 +406,57 @@ def dequantize_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.float32) -> torc
     if q.device.type != "cuda":
         raise RuntimeError("dequantize_mxfp4 needs a CUDA matrix (there is no CPU path)")
     rows, cols = q.shape
-    with _on_device(q.device):
-        out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    with _on_device(q.device.index):
+        out = q.codes.new_empty((rows, cols), dtype=dtype)
         _check(lib.xvram_b200_mxfp4_dequantize(_FEED_TYPES[dtype], rows, cols, q.codes.data_ptr(),
                                                q.scales.data_ptr(), out.data_ptr(), cols,
-                                               _stream(q.device)), "xvram_b200_mxfp4_dequantize")
+                                               _stream(q.device.index)),
+               "xvram_b200_mxfp4_dequantize")
     return out
 
 
-def _mxfp4_input(x, dtype, weights, what: str):
-    """(MXFP4 input, result type) of a product, its arguments checked."""
-    given = x.dtype if isinstance(x, torch.Tensor) else torch.float32
+def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) -> torch.Tensor:
+    """The product `call` of x and one or two MXFP4 weights, its arguments checked."""
+    quantised = isinstance(x, Mxfp4Matrix)
+    given = torch.float32 if quantised else x.dtype
     dtype = given if dtype is None else dtype
-    if dtype not in _FEED_TYPES or (isinstance(x, torch.Tensor) and x.dtype not in _FEED_TYPES):
+    if dtype not in _FEED_TYPES or given not in _FEED_TYPES:
         raise TypeError(f"{what} supports float16, bfloat16 and float32 (got {given} to {dtype})")
-    if len(x.shape) != 2 or any(not isinstance(w, Mxfp4Matrix) or w.shape[1] != x.shape[1] or
-                                w.shape != weights[0].shape for w in weights):
+    shape, device = x.shape, x.device
+    first = weights[0]
+    if len(shape) != 2 or any(not isinstance(w, Mxfp4Matrix) or w.shape[1] != shape[1] or
+                              w.shape[0] != first.shape[0] for w in weights):
         raise ValueError(f"{what} takes x (batch, in) and MXFP4 weights (out, in)")
-    if x.shape[1] == 0:
+    m, k = shape
+    n = first.shape[0]
+    if k == 0:
         raise ValueError(f"{what} needs at least one input feature")
-    if x.device.type != "cuda" or any(w.device != x.device for w in weights):
+    if device.type != "cuda" or any(w.codes.device != device for w in weights):
         raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
-    return (quantize_mxfp4(x) if isinstance(x, torch.Tensor) else x), dtype
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *biases)
+                                       if isinstance(t, torch.Tensor)):
+        raise RuntimeError(f"{what} has no gradient: detach its input and biases")
+    index = device.index
+    with _on_device(index):
+        if quantised:
+            src, ldx, codes, scales, like = 0, 0, x.codes.data_ptr(), x.scales.data_ptr(), x.codes
+        else:
+            like, ldx = _rows(x)
+            src = like.data_ptr()
+            size = m * ((k + 31) // 32) * 16
+            buffer = like.new_empty((size + (m + 127) // 128 * ((k + 127) // 128) * 512,),
+                                    dtype=torch.uint8)
+            codes = buffer.data_ptr()
+            scales = codes + size
+        out = like.new_empty((m, n), dtype=dtype)
+        b = [None if t is None else _check_bias(t, n, dtype, device, "bias") for t in biases]
+        last = weights[-1]
+        d = Mxfp4Product(_PRODUCT_SIZE, _FEED_TYPES[given], _FEED_TYPES[dtype], activation, m, n, k,
+                         src, ldx, codes, scales, first.codes.data_ptr(), last.codes.data_ptr(),
+                         first.scales.data_ptr(), last.scales.data_ptr(), _ptr(b[0]), _ptr(b[-1]),
+                         out.data_ptr(), n, _stream(index))
+        _check(call(ctypes.byref(d)), what)
+    return out
 
 
 def linear_mxfp4(x, weight: Mxfp4Matrix, bias: torch.Tensor | None = None, relu: bool = False,
@@ -419,17 +465,8 @@ def linear_mxfp4(x, weight: Mxfp4Matrix, bias: torch.Tensor | None = None, relu:
     operands, FP32 accumulation, rounded once.  x: (batch, in), a float tensor that is quantised
     here or an Mxfp4Matrix; weight: (out, in).  The result (and the bias) has `dtype`: x's type by
     default, float32 for an Mxfp4Matrix.  Inference only: no gradient."""
-    xq, dtype = _mxfp4_input(x, dtype, (weight,), "linear_mxfp4")
-    m, n, k = x.shape[0], weight.shape[0], x.shape[1]
-    with _on_device(xq.device):
-        out = torch.empty((m, n), dtype=dtype, device=xq.device)
-        bias = _check_bias(bias, n, out, "bias")
-        _check(lib.xvram_b200_mxfp4_linear(_FEED_TYPES[dtype], m, n, k, xq.codes.data_ptr(),
-                                           xq.scales.data_ptr(), weight.codes.data_ptr(),
-                                           weight.scales.data_ptr(), _ptr(bias), 1 if relu else 0,
-                                           out.data_ptr(), n, _stream(xq.device)),
-               "xvram_b200_mxfp4_linear")
-    return out
+    return _mxfp4_product(x, (weight,), (bias,), 1 if relu else 0, dtype, "linear_mxfp4",
+                          lib.xvram_b200_mxfp4_linear)
 
 
 def gated_linear_mxfp4(x, w_gate: Mxfp4Matrix, w_up: Mxfp4Matrix,
@@ -437,20 +474,8 @@ def gated_linear_mxfp4(x, w_gate: Mxfp4Matrix, w_up: Mxfp4Matrix,
                        activation: str = "silu", dtype: torch.dtype | None = None) -> torch.Tensor:
     """`gated_linear` over MXFP4 operands, with `linear_mxfp4`'s input and types: both products,
     the biases, the activation and the product of the two in one kernel.  No gradient."""
-    act = _activation(activation)
-    xq, dtype = _mxfp4_input(x, dtype, (w_gate, w_up), "gated_linear_mxfp4")
-    m, h, k = x.shape[0], w_gate.shape[0], x.shape[1]
-    with _on_device(xq.device):
-        out = torch.empty((m, h), dtype=dtype, device=xq.device)
-        bias_gate = _check_bias(bias_gate, h, out, "bias_gate")
-        bias_up = _check_bias(bias_up, h, out, "bias_up")
-        _check(lib.xvram_b200_mxfp4_gated(_FEED_TYPES[dtype], act, m, h, k, xq.codes.data_ptr(),
-                                          xq.scales.data_ptr(), w_gate.codes.data_ptr(),
-                                          w_gate.scales.data_ptr(), w_up.codes.data_ptr(),
-                                          w_up.scales.data_ptr(), _ptr(bias_gate), _ptr(bias_up),
-                                          out.data_ptr(), h, _stream(xq.device)),
-               "xvram_b200_mxfp4_gated")
-    return out
+    return _mxfp4_product(x, (w_gate, w_up), (bias_gate, bias_up), _activation(activation), dtype,
+                          "gated_linear_mxfp4", lib.xvram_b200_mxfp4_gated)
 
 
 class HostGemm:
