@@ -414,6 +414,20 @@ typedef struct xvram_b200_gated_v1 {
   uint64_t stream;
 } xvram_b200_gated_v1;
 
+/* Copies of up to XVRAM_B200_PACK_MAX matrices with rows padded to whole 16 bytes (zeros), in
+ * one launch, for operands whose alignment the tensor-core kernels do not take.  Sources start
+ * at any element; dst is 16-byte aligned and ld_dst x the element size a multiple of 16.  One
+ * data type (FP16, BF16 or FP32) for all. */
+#define XVRAM_B200_PACK_MAX 4
+typedef struct xvram_b200_pack_v1 {
+  uint64_t src, dst;
+  int64_t ld_src, ld_dst; /* elements */
+  int64_t rows, cols;
+} xvram_b200_pack_v1;
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_pack_rows(uint32_t data_type,
+                                                          const xvram_b200_pack_v1* items,
+                                                          uint32_t count, uint64_t stream);
+
 /* Bytes of workspace the forward (backward = 0) or backward pass of this problem needs; only
  * the type, the sizes, the transpositions and whether pre_gate is set are read.  0 for an
  * invalid problem. */

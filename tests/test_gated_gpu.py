@@ -78,3 +78,32 @@ def test_more_tiles_than_the_gpu_holds(kind):
     """Each resident CTA pair walks several tiles, in the forward and in both gradient products."""
     m, h, k = 2200, 1500, 2050
     check_gradients(problem(kind, m, h, k, 40), "gelu_tanh", fu.normal((m, h), kind, 41))
+
+
+def layouts(t):
+    """The same matrix as rows, as columns, inside a larger one at an odd place, and with no
+    contiguous axis."""
+    r, c = t.shape
+    big = t.new_zeros((r + 2, c + 3))
+    big[1:r + 1, 1:c + 1] = t
+    tall = t.new_zeros((c + 1, r + 5))
+    tall[1:, 3:r + 3] = t.t()
+    wide = t.new_zeros((r, 2 * c))
+    wide[:, ::2] = t
+    return [t, t.t().contiguous().t(), big[1:r + 1, 1:c + 1], tall[1:, 3:r + 3].t(), wide[:, ::2]]
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 56), (200, 72, 64), (1, 9, 5), (70, 1, 33), (40, 8, 1)])
+@pytest.mark.parametrize("kind", TYPES)
+def test_every_operand_layout(kind, shape):
+    m, h, k = shape
+    x, wg, wu, bg, bu = problem(kind, m, h, k, 50)
+    dh = fu.normal((m, h), kind, 51)
+    for xv in layouts(x):
+        check_gradients((xv, wg, wu, bg, bu), "silu", dh)
+    for g, u in zip(layouts(wg), layouts(wu)):
+        check_forward((x, g, u, bg, bu), "silu")
+        check_gradients((x, g, u, bg, bu), "silu", dh)
+    check_gradients((x, wg, layouts(wu)[1], bg, bu), "silu", dh)  # stored in different ways
+    for dhv in layouts(dh)[1:] + [dh[:1].expand(m, h)]:
+        check_gradients((x, wg, wu, bg, bu), "silu", dhv)

@@ -98,6 +98,13 @@ class Gated(C.Structure):
                 ("ld_pre", i64), ("workspace", u64), ("workspace_bytes", u64), ("stream", u64)]
 
 
+class Pack(C.Structure):
+    """xvram_b200_pack_v1 (include/xvram_b200.h)."""
+
+    _fields_ = [("src", u64), ("dst", u64), ("ld_src", i64), ("ld_dst", i64), ("rows", i64),
+                ("cols", i64)]
+
+
 class Mxfp4Product(C.Structure):
     """xvram_b200_mxfp4_product_v1 (include/xvram_b200.h)."""
 
@@ -183,6 +190,8 @@ def _load() -> C.CDLL:
     gated = C.POINTER(Gated)
     lib.xvram_b200_gated_workspace_bytes.argtypes = [gated, u32]
     lib.xvram_b200_gated_workspace_bytes.restype = u64
+    lib.xvram_b200_pack_rows.argtypes = [u32, C.POINTER(Pack), u32, u64]
+    lib.xvram_b200_pack_rows.restype = u32
     lib.xvram_b200_gated_forward.argtypes = [gated, u64, i64]
     lib.xvram_b200_gated_forward.restype = u32
     lib.xvram_b200_gated_backward.argtypes = [gated, u64, i64, u64, i64, u64, u64, i64, u64, u64]
@@ -249,6 +258,7 @@ EXPORTED = (
     "xvram_b200_gemm_typed_workspace_bytes",
     "xvram_b200_gemm_device_typed",
     "xvram_b200_gated_workspace_bytes",
+    "xvram_b200_pack_rows",
     "xvram_b200_gated_forward",
     "xvram_b200_gated_backward",
     "xvram_b200_mxfp4_bytes",

@@ -53,7 +53,7 @@ struct Params {
   int tiles_m, tiles_n, batches;
   int a_mn, b_mn;         // 16-bit operands stored M-/N-major
   int act, relu;
-  int vec_out;            // output rows allow 16-byte accesses
+  int unit;               // widest access the output rows allow, in bytes (store_unit)
   uint32_t idesc;
   const void *bias0, *bias1;
   void* out[2];           // by batch
@@ -148,20 +148,37 @@ __device__ __forceinline__ void stage_mxf4(const Params& p, uint32_t d, uint32_t
 }
 
 // ---------------------------------------------------------------- activations
-// Fast: for results rounded to 16 bits; __expf and __fdividef are within a few 2^-22 of the
-// quotient's value, far below half a step of either type (2^-11, 2^-8).  Otherwise the
-// library functions, for FP32 results.
-template <bool FAST>
-__device__ __forceinline__ float exp_of(float v) {
-  return FAST ? __expf(v) : expf(v);
-}
+// FAST: for results rounded to 16 bits.  __expf(x) is off by about (2 + 1.2 |x|) 2^-23 relative and
+// __fdividef by 2^-22: below 2^-19 for |x| <= 20, where half a step of the types is 2^-11 and
+// 2^-8.  Otherwise the library functions, for FP32 results.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float v) {
   // exp(-v) overflows to infinity for very negative v: 1 / inf = 0, as it should be.
   return FAST ? __fdividef(1.0f, 1.0f + __expf(-v)) : 1.0f / (1.0f + expf(-v));
 }
-// Phi(v), the standard normal distribution function, without cancellation for v << 0.
-__device__ __forceinline__ float normal_cdf(float v) { return 0.5f * erfcf(-v * 0.70710678118654752f); }
+// Phi(v) = erfc(-v / sqrt 2) / 2, the standard normal distribution function, without
+// cancellation for v << 0, and e = exp(-v^2 / 2), which its slope needs too.  FAST: with
+// z = |v| / sqrt 2, erfc(z) = exp(-z^2) t P(t), t = 1 / (1 + 0.455 z); P is the least-maximum fit of
+// degree 7 to exp(z^2) erfc(z) / t over z >= 0 (relative error 8e-7 in FP32, all z).
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float v, float& e) {
+  e = FAST ? __expf(-0.5f * v * v) : expf(-0.5f * v * v);
+  if constexpr (FAST) {
+    const float t = __fdividef(1.0f, fmaf(0.455f * 0.70710678118654752f, fabsf(v), 1.0f));
+    float s = 0.06859361380338669f;
+    s = fmaf(s, t, -0.238698810338974f);
+    s = fmaf(s, t, 0.19744166731834412f);
+    s = fmaf(s, t, 0.0389687679708004f);
+    s = fmaf(s, t, 0.19179636240005493f);
+    s = fmaf(s, t, 0.2283932864665985f);
+    s = fmaf(s, t, 0.2568010985851288f);
+    s = fmaf(s, t, 0.25670450925827026f);
+    const float half = 0.5f * s * t * e;
+    return v < 0.0f ? half : 1.0f - half; // a NaN stays one
+  } else {
+    return 0.5f * erfcf(-v * 0.70710678118654752f);
+  }
+}
 
 constexpr float kTanhC = 0.79788456080286536f; // sqrt(2 / pi)
 constexpr float kTanhK = 0.044715f;
@@ -172,8 +189,10 @@ template <int ACT, bool FAST>
 __device__ __forceinline__ float act_of(float v) {
   if constexpr (ACT == kSilu)
     return v * sigmoid<FAST>(v);
-  else if constexpr (ACT == kGelu)
-    return v * normal_cdf(v);
+  else if constexpr (ACT == kGelu) {
+    float e;
+    return v * normal_cdf<FAST>(v, e);
+  }
   else if constexpr (ACT == kGeluTanh)
     return v * sigmoid<FAST>(2.0f * kTanhC * (v + kTanhK * v * v * v));
   else if constexpr (ACT == kRelu)
@@ -190,9 +209,10 @@ __device__ __forceinline__ void act_and_slope(float v, float& a, float& d) {
     a = v * q;
     d = fmaf(a, 1.0f - q, q);
   } else if constexpr (ACT == kGelu) {
-    const float q = normal_cdf(v);
+    float e;
+    const float q = normal_cdf<FAST>(v, e);
     a = v * q;
-    d = fmaf(v * 0.39894228040143268f, exp_of<FAST>(-0.5f * v * v), q);
+    d = fmaf(v * 0.39894228040143268f, e, q);
   } else if constexpr (ACT == kGeluTanh) {
     const float q = sigmoid<FAST>(2.0f * kTanhC * (v + kTanhK * v * v * v));
     a = v * q;
@@ -306,12 +326,13 @@ __device__ __forceinline__ void load_accumulator(uint32_t t_row, int half, float
 }
 
 // A warp's 32 rows x 128 bytes of results, row per lane, to global memory in whole lines:
-// through `block` (shared memory, 16-byte chunks swizzled by the row), then 8 lanes per row.
+// through `block` (shared memory, 16-byte chunks swizzled by the row), then 8 lanes per row
+// where rows are 16-byte aligned (unit 16), else one row at a time by 4 bytes or by elements.
 constexpr int kStageBlock = 32 * 128;
 template <class T, int N>
 __device__ __forceinline__ void store_block(unsigned char* block, const float (&v)[N], int from,
                                             T* out, long long ld, int row0, int col, int m, int n,
-                                            bool vec) {
+                                            int unit) {
   constexpr int per = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -324,23 +345,81 @@ __device__ __forceinline__ void store_block(unsigned char* block, const float (&
         *reinterpret_cast<const uint4*>(t);
   }
   __syncwarp();
-  const int c = lane & 7, cc = col + c * per;
+  if (unit == 16) {
+    const int c = lane & 7, cc = col + c * per;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    const uint4 raw = *reinterpret_cast<const uint4*>(block + r * 128 + ((c ^ (r & 7)) * 16));
-    if (row0 + r < m) {
-      T* dst = out + static_cast<long long>(row0 + r) * ld + cc;
-      if (vec && cc + per <= n) {
-        *reinterpret_cast<uint4*>(dst) = raw;
-      } else {
-        const T* t = reinterpret_cast<const T*>(&raw);
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      const uint4 raw = *reinterpret_cast<const uint4*>(block + r * 128 + ((c ^ (r & 7)) * 16));
+      if (row0 + r < m) {
+        T* dst = out + static_cast<long long>(row0 + r) * ld + cc;
+        if (cc + per <= n) {
+          *reinterpret_cast<uint4*>(dst) = raw;
+        } else {
+          const T* t = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-        for (int j = 0; j < per; ++j)
-          if (cc + j < n)
-            dst[j] = t[j];
+          for (int j = 0; j < per; ++j)
+            if (cc + j < n)
+              dst[j] = t[j];
+        }
       }
     }
+  } else {
+    const int rows = min(32, m - row0);
+    constexpr int pair = 4 / sizeof(T); // elements of 4 bytes
+    T* dst = out + static_cast<long long>(row0) * ld + col;
+    const int left = n - col;
+    if (unit == 4) {
+      const int e = lane * pair;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, dst += ld) {
+        const uint32_t raw = *reinterpret_cast<const uint32_t*>(
+            block + r * 128 + (((lane >> 2) ^ (r & 7)) * 16) + (lane & 3) * 4);
+        if (e + pair <= left)
+          *reinterpret_cast<uint32_t*>(dst + e) = raw;
+        else if (e < left)
+          dst[e] = *reinterpret_cast<const T*>(&raw);
+      }
+    } else {
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, dst += ld) {
+#pragma unroll
+        for (int j = 0; j < pair; ++j) {
+          const int e = lane + 32 * j, b = e * static_cast<int>(sizeof(T));
+          if (e < left)
+            dst[e] = *reinterpret_cast<const T*>(block + r * 128 + (((b >> 4) ^ (r & 7)) * 16) +
+                                                 (b & 15));
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// The widest access that every row of `base` allows: 16 bytes, 4, or an element's.
+template <class T>
+inline int store_unit(const void* base, long long ld) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(ld * sizeof(T));
+  return a % 16 == 0 ? 16 : a % 4 == 0 ? 4 : static_cast<int>(sizeof(T));
+}
+
+// v[from + i] += bias[col + i] for i < N: read once per warp, then broadcast from shared memory.
+template <class T, int COUNT, int N>
+__device__ __forceinline__ void add_bias_rows(unsigned char* block, const void* bias, int col, int n,
+                                              float (&v)[N]) {
+  if (!bias)
+    return;
+  const T* b = static_cast<const T*>(bias);
+  float* shared = reinterpret_cast<float*>(block);
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < COUNT; i += 32)
+    shared[i + lane] = col + i + lane < n ? to_float(b[col + i + lane]) : 0.0f;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < COUNT; i += 4) {
+    const float4 t = *reinterpret_cast<const float4*>(shared + i);
+    v[i] += t.x, v[i + 1] += t.y, v[i + 2] += t.z, v[i + 3] += t.w;
   }
   __syncwarp();
 }
@@ -360,21 +439,21 @@ __device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], in
       g[i] = v[i];
       u[i] = v[64 + i];
     }
-    add_bias<T>(p.bias0, col, p.n, g);
-    add_bias<T>(p.bias1, col, p.n, u);
+    add_bias_rows<T, 64>(block, p.bias0, col, p.n, g);
+    add_bias_rows<T, 64>(block, p.bias1, col, p.n, u);
     if (p.save_gate) {
 #pragma unroll
       for (int i = 0; i < 64; i += 32) {
-        store_block(block, g, i, p.save_gate, p.lds, row0, col + i, p.m, p.n, true);
-        store_block(block, u, i, p.save_up, p.lds, row0, col + i, p.m, p.n, true);
+        store_block(block, g, i, p.save_gate, p.lds, row0, col + i, p.m, p.n, 16);
+        store_block(block, u, i, p.save_up, p.lds, row0, col + i, p.m, p.n, 16);
       }
     }
     gate<sizeof(T) == 2>(p.act, g, u);
 #pragma unroll
     for (int i = 0; i < 64; i += kBlockCols)
-      store_block(block, g, i, out, p.ldo, row0, col + i, p.m, p.n, p.vec_out != 0);
+      store_block(block, g, i, out, p.ldo, row0, col + i, p.m, p.n, p.unit);
   } else {
-    add_bias<T>(p.bias0, col, p.n, v);
+    add_bias_rows<T, 128>(block, p.bias0, col, p.n, v);
     if (p.relu) {
 #pragma unroll
       for (int i = 0; i < 128; ++i)
@@ -382,7 +461,7 @@ __device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], in
     }
 #pragma unroll
     for (int i = 0; i < 128; i += kBlockCols)
-      store_block(block, v, i, out, p.ldo, row0, col + i, p.m, p.n, p.vec_out != 0);
+      store_block(block, v, i, out, p.ldo, row0, col + i, p.m, p.n, p.unit);
   }
 }
 

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         v[j] = act_of<kRelu, true>(v[j]);
     }
     T* dst = out + r * p.ldo + col;
-    if (p.vec_out && col + 4 <= p.n) {
+    if (p.unit == 16 && col + 4 <= p.n) {
       alignas(16) T t[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)

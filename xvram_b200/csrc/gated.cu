@@ -265,7 +265,7 @@ cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStre
   p.bias1 = q.bias_up;
   p.out[0] = p.out[1] = out;
   p.ldo = ldo;
-  p.vec_out = ldo % 8 == 0 && aligned16(out);
+  p.unit = store_unit<T>(out, ldo);
   p.save_gate = q.pre_gate;
   p.save_up = q.pre_up;
   p.lds = q.ld_pre;
@@ -306,7 +306,7 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.k_split = per;
     p.out[0] = p.out[1] = d.dx;
     p.ldo = d.lddx;
-    p.vec_out = d.lddx % 8 == 0 && aligned16(d.dx);
+    p.unit = store_unit<T>(d.dx, d.lddx);
     if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, stream);
         e != cudaSuccess)
       return e;
@@ -326,12 +326,54 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[0] = d.dw_gate ? d.dw_gate : d.dw_up;
     p.out[1] = d.dw_up;
     p.ldo = d.ld_dw;
-    p.vec_out = d.ld_dw % 8 == 0 && aligned16(p.out[0]) && aligned16(p.out[1]);
+    p.unit = std::min(store_unit<T>(p.out[0], d.ld_dw), store_unit<T>(p.out[1], d.ld_dw));
     if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, stream);
         e != cudaSuccess)
       return e;
   }
   return cudaSuccess;
+}
+
+// ---------------------------------------------------------------- padded copies
+// Rows of unaligned 16- or 32-bit matrices to rows of whole 16 bytes, up to kPackMax matrices in a
+// launch.  A thread writes 16 bytes; where the source is only 2-byte aligned it reads the 4-byte
+// words around them (each holds a byte of the row, so no word lies outside the allocation).
+struct PackParams {
+  PackItem item[kPackMax];
+  long long first[kPackMax + 1]; // first 16-byte chunk of each matrix
+  int count;
+};
+
+__global__ void __launch_bounds__(256) pack_rows_kernel(const PackParams p, int size) {
+  const long long total = p.first[p.count];
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    int k = 0;
+    while (k + 1 < p.count && i >= p.first[k + 1])
+      ++k;
+    const PackItem& t = p.item[k];
+    const long long chunks = (t.cols * size + 15) / 16, j = i - p.first[k];
+    const long long r = j / chunks;
+    const long long b = (j - r * chunks) * 16; // byte in the row
+    const int bytes = static_cast<int>(min(16ll, t.cols * size - b));
+    const char* src = static_cast<const char*>(t.src) + r * t.lds * size + b;
+    const uint32_t* w =
+        reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t{3});
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 2); // bytes
+    uint32_t v[5] = {};
+#pragma unroll
+    for (int q = 0; q < 5; ++q)
+      if (4 * q < bytes + shift)
+        v[q] = w[q];
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      o[q] = shift ? __funnelshift_r(v[q], v[q + 1], 16) : v[q];
+      const int left = bytes - 4 * q; // bytes of this word inside the row
+      o[q] &= left >= 4 ? 0xffffffffu : left > 0 ? 0xffffu : 0u;
+    }
+    *reinterpret_cast<uint4*>(static_cast<char*>(t.dst) + r * t.ldd * size + b) =
+        make_uint4(o[0], o[1], o[2], o[3]);
+  }
 }
 
 // ---------------------------------------------------------------- few rows
@@ -518,6 +560,23 @@ cudaError_t gated_backward(const GatedProblem& q, const GatedGradients& d, void*
   case GatedType::bf16: return backward_16<__nv_bfloat16>(q, d, ws, stream);
   default: return backward_f32(q, d, ws, stream);
   }
+}
+
+cudaError_t pack_rows(const PackItem* items, int count, int element_size, cudaStream_t stream) {
+  if (count < 1 || count > kPackMax || (element_size != 2 && element_size != 4))
+    return cudaErrorInvalidValue;
+  PackParams p{};
+  p.count = count;
+  for (int i = 0; i < count; ++i) {
+    p.item[i] = items[i];
+    p.first[i + 1] = p.first[i] + items[i].rows * ((items[i].cols * element_size + 15) / 16);
+  }
+  if (p.first[count] == 0)
+    return cudaSuccess;
+  const long long blocks =
+      std::min<long long>((p.first[count] + 255) / 256, 16ll * tc::sm_count());
+  pack_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p, element_size);
+  return cudaGetLastError();
 }
 
 cudaError_t read_and_clear_kernel_error_gated(unsigned int* out, cudaStream_t stream) {

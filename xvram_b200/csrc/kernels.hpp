@@ -129,6 +129,17 @@ struct GatedGradients {
   long long ld_dw = 0;
   void *db_gate = nullptr, *db_up = nullptr;
 };
+// Copies of up to kPackMax matrices of 2- or 4-byte elements, whose rows start at any element, with
+// rows padded to whole 16 bytes (the padding is zeroed): dst 16-byte aligned, ldd * size a
+// multiple of 16.
+constexpr int kPackMax = 4;
+struct PackItem {
+  const void* src = nullptr;
+  void* dst = nullptr;
+  long long lds = 0, ldd = 0, rows = 0, cols = 0;
+};
+cudaError_t pack_rows(const PackItem* items, int count, int element_size, cudaStream_t stream);
+
 uint64_t gated_partial_bytes(int m, int h);
 uint64_t gated_workspace_bytes(const GatedProblem& q, bool backward);
 cudaError_t gated_forward(const GatedProblem& q, void* out, long long ldo, void* workspace,

@@ -209,7 +209,7 @@ cudaError_t product(const Mxfp4Product& q, bool after, cudaStream_t stream) {
   p.bias1 = q.bias[1];
   p.out[0] = p.out[1] = q.out;
   p.ldo = q.ldo;
-  p.vec_out = vec_rows<T>(q.out, q.ldo);
+  p.unit = store_unit<T>(q.out, q.ldo);
   p.timeout_ns = kernel_wait_limit_ns();
   p.idesc = idesc_mxf4(split ? 128 : 256, 256);
   return split ? launch_split<Kind::mxf4, E, T>(maps, p, after, stream)

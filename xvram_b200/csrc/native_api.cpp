@@ -521,6 +521,27 @@ xvram_b200_gated_workspace_bytes(const xvram_b200_gated_v1* problem, uint32_t ba
   return gated_workspace_bytes(q, backward != 0);
 }
 
+XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_pack_rows(uint32_t data_type,
+                                                          const xvram_b200_pack_v1* items,
+                                                          uint32_t count, uint64_t stream) {
+  static_assert(kPackMax == XVRAM_B200_PACK_MAX, "one limit");
+  if (data_type > XVRAM_DATA_FP32 || !items || count < 1 || count > XVRAM_B200_PACK_MAX)
+    return XVRAM_STATUS_INVALID_ARGUMENT;
+  const int size = data_type == XVRAM_DATA_FP32 ? 4 : 2;
+  PackItem list[kPackMax];
+  for (uint32_t i = 0; i < count; ++i) {
+    const xvram_b200_pack_v1& t = items[i];
+    if (t.rows < 0 || t.cols < 0 || t.rows > INT32_MAX || t.cols > INT32_MAX ||
+        t.ld_dst < t.cols || t.ld_src < 0)
+      return XVRAM_STATUS_INVALID_ARGUMENT;
+    if (t.rows && t.cols && (!t.src || !t.dst || !element_aligned(t.src, data_type) ||
+                             t.dst % 16 || t.ld_dst * size % 16))
+      return XVRAM_STATUS_INVALID_ARGUMENT;
+    list[i] = {pointer(t.src), pointer(t.dst), t.ld_src, t.ld_dst, t.rows, t.cols};
+  }
+  return from_cuda(pack_rows(list, static_cast<int>(count), size, as_stream(stream)));
+}
+
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_forward(const xvram_b200_gated_v1* problem,
                                                               uint64_t out, int64_t ld_out) {
   GatedProblem q;

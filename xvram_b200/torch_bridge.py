@@ -45,7 +45,7 @@ import torch
 
 from . import device as xd
 from . import sdk
-from ._native import Gated, Mxfp4Product, lib
+from ._native import Gated, Mxfp4Product, Pack, lib
 
 _TF32X3 = 3
 _TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32: sdk.FP32,
@@ -141,9 +141,10 @@ _FEED_TYPES = {torch.float16: sdk.FP16, torch.bfloat16: sdk.BF16, torch.float32:
 
 
 def _activation(name: str) -> int:
-    if name not in ACTIVATIONS:
+    act = ACTIVATIONS.get(name)
+    if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)} (got {name!r})")
-    return ACTIVATIONS[name]
+    return act
 
 
 def _on_device(index: int):
@@ -161,23 +162,45 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _operand(x: torch.Tensor, aligned: bool):
-    """(tensor, leading dimension, transposed): x itself where the kernels can read it, else a
-    copy whose rows are padded to 16 bytes.  `aligned`: rows must be multiples of 16 bytes."""
-    r, c = x.shape
+def _operand(x: torch.Tensor, r: int, c: int, per: int, aligned: bool):
+    """(leading dimension, transposed, padded) of x as the kernels read it.  padded: x must be
+    copied with rows (or, transposed, columns) of whole 16 bytes first.  `per`: elements in 16
+    bytes; `aligned`: rows must be multiples of them.  (None, ...): neither rows nor columns are
+    contiguous."""
     s0, s1 = x.stride()
-    per = 16 // x.element_size()
-    if r == 1 and s1 == 1:  # one row's stride is never used
-        s0 = (c + per - 1) // per * per
-    if not aligned or x.data_ptr() % 16 == 0:
-        if s1 == 1 and s0 >= c and not (aligned and s0 % per):
-            return x, s0, 0
-        if s0 == 1 and s1 >= r and not (aligned and s1 % per):
-            return x, s1, 1
-    ld = (c + per - 1) // per * per
-    y = torch.empty((r, ld), dtype=x.dtype, device=x.device)[:, :c]
-    y.copy_(x)
-    return y, ld, 0
+    if s1 == 1 and (s0 >= c or r == 1):
+        if r == 1:  # one row's stride is never used
+            s0 = (c + per - 1) // per * per
+        if not aligned or (s0 % per == 0 and x.data_ptr() % 16 == 0):
+            return s0, 0, False
+        return (c + per - 1) // per * per, 0, True
+    if s0 == 1 and (s1 >= r or c == 1):
+        if c == 1:
+            s1 = (r + per - 1) // per * per
+        if not aligned or (s1 % per == 0 and x.data_ptr() % 16 == 0):
+            return s1, 1, False
+        return (r + per - 1) // per * per, 1, True
+    return None, 0, False
+
+
+def _pack(padded: list, like: torch.Tensor, per: int, kind: int, index: int):
+    """Copies (tensor, rows, leading dimension, transposed) with padded rows into one buffer, in
+    one launch: (buffer, each copy's element offset)."""
+    offsets, end = [], 0
+    for _, rows, ld, _ in padded:
+        offsets.append(end)
+        end += rows * ld
+    buffer = like.new_empty(end)
+    base, size = buffer.data_ptr(), 16 // per
+    items = (Pack * len(padded))()
+    for item, (x, rows, ld, transposed), off in zip(items, padded, offsets):
+        s0, s1 = x.stride()
+        r, c = x.shape
+        item.src, item.dst, item.ld_dst = x.data_ptr(), base + off * size, ld
+        item.ld_src, item.rows, item.cols = (s1, c, r) if transposed else (s0, r, c)
+    _check(lib.xvram_b200_pack_rows(kind, items, len(padded), _stream(index)),
+           "xvram_b200_pack_rows")
+    return buffer, offsets
 
 
 _GATED_SIZE = ctypes.sizeof(Gated)
@@ -190,87 +213,99 @@ def _check_bias(b: torch.Tensor, h: int, dtype: torch.dtype, device: torch.devic
     return b.contiguous()
 
 
-def _check_gated(x, w_gate, w_up) -> None:
-    if x.dtype not in _FEED_TYPES or w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
+def _check_gated(x, w_gate, w_up, dtype: torch.dtype, device: torch.device) -> None:
+    if dtype not in _FEED_TYPES or w_gate.dtype != dtype or w_up.dtype != dtype:
         raise TypeError("gated_linear supports float16, bfloat16 and float32 matrices of one type "
-                        f"(got {x.dtype}, {w_gate.dtype} and {w_up.dtype})")
-    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or \
-            x.shape[1] != w_gate.shape[1]:
-        raise ValueError(f"x (batch, in) and two (out, in) weights expected (got {tuple(x.shape)}, "
-                         f"{tuple(w_gate.shape)} and {tuple(w_up.shape)})")
-    if x.shape[1] == 0:
+                        f"(got {dtype}, {w_gate.dtype} and {w_up.dtype})")
+    xs, gs = x.shape, w_gate.shape
+    if len(xs) != 2 or len(gs) != 2 or gs != w_up.shape or xs[1] != gs[1]:
+        raise ValueError(f"x (batch, in) and two (out, in) weights expected (got {tuple(xs)}, "
+                         f"{tuple(gs)} and {tuple(w_up.shape)})")
+    if xs[1] == 0:
         raise ValueError("gated_linear needs at least one input feature")
-    if x.device.type != "cuda":
+    if device.type != "cuda":
         raise RuntimeError("gated_linear needs CUDA tensors (there is no CPU path)")
-    if w_gate.device != x.device or w_up.device != x.device:
+    if w_gate.device != device or w_up.device != device:
         raise ValueError("x and the weights must be on the same device")
 
 
-@dataclasses.dataclass
 class GatedSaved:
     """What `gated_linear_backward` needs of a forward pass: the operands as the kernels read
-    them and the FP32 pre-activations."""
-    x: torch.Tensor
-    w_gate: torch.Tensor
-    w_up: torch.Tensor
-    pre_gate: torch.Tensor
-    pre_up: torch.Tensor
-    activation: str
+    them (x, w_gate, w_up, or the buffer that holds their padded copies) and the FP32
+    pre-activations (2, batch, out), with their layout."""
+    __slots__ = ("tensors", "layout")
 
-
-def _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act: int, backward: bool):
-    """The call's descriptor and the tensors it points to, which must outlive the call."""
-    (m, k), h = x.shape, w_gate.shape[0]
-    # The float32 GEMM reads any operand, but unaligned ones several times slower than it takes to
-    # copy them; the few-rows kernel reads them at full speed.
-    aligned = x.dtype != torch.float32 or backward or m > 32
-    xo, ldx, xt = _operand(x, aligned)
-    go, ldg, gt = _operand(w_gate, aligned)
-    uo, ldu, ut = _operand(w_up, aligned)
-    if gt != ut:  # one weight row-major, the other transposed: bring the latter to rows
-        if gt:
-            go, ldg, gt = _operand(w_gate.contiguous(), aligned)
-        else:
-            uo, ldu, ut = _operand(w_up.contiguous(), aligned)
-    d = Gated(_GATED_SIZE, _FEED_TYPES[x.dtype], act, xt, gt, 0, m, h, k, xo.data_ptr(),
-              go.data_ptr(), uo.data_ptr(), ldx, ldg, ldu, _ptr(bias_gate), _ptr(bias_up),
-              _ptr(pre_gate), _ptr(pre_up), 0 if pre_gate is None else pre_gate.stride(0), 0, 0,
-              _stream(x.device.index))
-    return d, (xo, go, uo)
-
-
-def _gated_workspace(d, backward: int, device: torch.device):
-    need = lib.xvram_b200_gated_workspace_bytes(ctypes.byref(d), backward)
-    if not need:
-        return None
-    ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
-    d.workspace = (ws.data_ptr() + 255) // 256 * 256
-    d.workspace_bytes = need
-    return ws
+    def __init__(self, tensors, layout):
+        self.tensors, self.layout = tensors, layout
 
 
 def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: bool):
     act = _activation(activation)
-    _check_gated(x, w_gate, w_up)
-    m, h = x.shape[0], w_gate.shape[0]
+    dtype, device = x.dtype, x.device
+    _check_gated(x, w_gate, w_up, dtype, device)
+    kind, index = _FEED_TYPES[dtype], device.index
+    (m, k), h = x.shape, w_gate.shape[0]
     if bias_gate is not None:
-        bias_gate = _check_bias(bias_gate, h, x.dtype, x.device, "bias_gate")
+        bias_gate = _check_bias(bias_gate, h, dtype, device, "bias_gate")
     if bias_up is not None:
-        bias_up = _check_bias(bias_up, h, x.dtype, x.device, "bias_up")
-    with _on_device(x.device.index):
+        bias_up = _check_bias(bias_up, h, dtype, device, "bias_up")
+    per = 4 if kind == sdk.FP32 else 8
+    # The float32 GEMM reads any operand, but unaligned ones several times slower than it takes to
+    # copy them; its few-rows kernel reads them at full speed.  The backward needs them aligned.
+    aligned = kind != sdk.FP32 or keep or m > 32
+    with _on_device(index):
+        ldx, xt, px = _operand(x, m, k, per, aligned)
+        ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
+        ldu, ut, pu = _operand(w_up, h, k, per, aligned)
+        if ldx is None or ldg is None or ldu is None or gt != ut:
+            # Neither rows nor columns contiguous, or weights stored in different ways.
+            x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+            ldx, xt, px = _operand(x, m, k, per, aligned)
+            ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
+            ldu, ut, pu = _operand(w_up, h, k, per, aligned)
+        ox = og = ou = 0
+        if px or pg or pu:
+            padded = [t for p, t in ((px, (x, k if xt else m, ldx, xt)),
+                                     (pg, (w_gate, k if gt else h, ldg, gt)),
+                                     (pu, (w_up, k if gt else h, ldu, gt))) if p]
+            buffer, offsets = _pack(padded, x, per, kind, index)
+            if px:
+                x, ox = buffer, offsets.pop(0)
+            if pg:
+                w_gate, og = buffer, offsets.pop(0)
+            if pu:
+                w_up, ou = buffer, offsets.pop(0)
         out = x.new_empty((m, h))
-        pre_gate = pre_up = None
+        pre, pg0, pu0, ldp = None, 0, 0, 0
         if keep:
-            pre_gate, pre_up = torch.empty((2, m, (h + 3) // 4 * 4), dtype=torch.float32,
-                                           device=x.device).unbind()
-        d, operands = _gated_desc(x, w_gate, w_up, bias_gate, bias_up, pre_gate, pre_up, act,
-                                  False)
-        ws = None
-        if x.dtype == torch.float32:
-            ws = _gated_workspace(d, 0, x.device)  # noqa: F841  (alive until the launch)
-        _check(lib.xvram_b200_gated_forward(ctypes.byref(d), out.data_ptr(), h),
-               "xvram_b200_gated_forward")
-    return out, (GatedSaved(*operands, pre_gate, pre_up, activation) if keep else None)
+            ldp = (h + 3) // 4 * 4
+            pre = x.new_empty((2, m, ldp), dtype=torch.float32)
+            pg0 = pre.data_ptr()
+            pu0 = pg0 + m * ldp * 4
+        size = 16 // per
+        d = Gated(_GATED_SIZE, kind, act, xt, gt, 0, m, h, k, x.data_ptr() + ox * size,
+                  w_gate.data_ptr() + og * size, w_up.data_ptr() + ou * size, ldx, ldg, ldu,
+                  0 if bias_gate is None else bias_gate.data_ptr(),
+                  0 if bias_up is None else bias_up.data_ptr(), pg0, pu0, ldp, 0, 0,
+                  _stream(index))
+        ws = _gated_workspace(d, 0, x) if kind == sdk.FP32 else None  # noqa: F841  (alive here)
+        st = lib.xvram_b200_gated_forward(ctypes.byref(d), out.data_ptr(), h)
+        if st:
+            _check(st, "xvram_b200_gated_forward")
+    if not keep:
+        return out, None
+    return out, GatedSaved((x, w_gate, w_up, pre), (kind, act, xt, gt, m, h, k, ox, og, ou, ldx, ldg,
+                                                    ldu, ldp, dtype, device))
+
+
+def _gated_workspace(d, backward: int, like: torch.Tensor):
+    need = lib.xvram_b200_gated_workspace_bytes(ctypes.byref(d), backward)
+    if not need:
+        return None
+    ws = like.new_empty((need + 256,), dtype=torch.uint8)
+    d.workspace = (ws.data_ptr() + 255) // 256 * 256
+    d.workspace_bytes = need
+    return ws
 
 
 def gated_linear_forward(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu"):
@@ -285,39 +320,42 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     """Gradients (dx, dw_gate, dw_up, db_gate, db_up) of the block from dh = dL/dh; those that
     `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
     pre-activations are rounded to the type once, as the tensor cores' operands."""
-    x, w_gate, w_up = saved.x, saved.w_gate, saved.w_up
-    (m, k), h = x.shape, w_gate.shape[0]
-    if dh.shape != (m, h) or dh.dtype != x.dtype or dh.device != x.device:
-        raise ValueError(f"dh must be a ({m}, {h}) {x.dtype} tensor on {x.device}")
-    with torch.no_grad(), _on_device(x.device.index):
-        if dh.stride(1) != 1 or dh.stride(0) < h:
-            dh = dh.contiguous()
-        shapes = ((m, k), (h, k), (h, k), (h,), (h,))
-        grads = [torch.empty(s, dtype=x.dtype, device=x.device) if n else None
-                 for s, n in zip(shapes, needs)]
-        d, operands = _gated_desc(x, w_gate, w_up, None, None, saved.pre_gate, saved.pre_up,
-                                  _activation(saved.activation), True)
-        ws = _gated_workspace(d, 1, x.device)  # noqa: F841
-        dx, dwg, dwu, dbg, dbu = (_ptr(g) for g in grads)
-        _check(lib.xvram_b200_gated_backward(ctypes.byref(d), dh.data_ptr(), max(dh.stride(0), h),
-                                             dx, k, dwg, dwu, k, dbg, dbu),
+    kind, act, xt, wt, m, h, k, ox, og, ou, ldx, ldg, ldu, ldp, dtype, device = saved.layout
+    x, w_gate, w_up, pre = saved.tensors
+    if dh.shape != (m, h) or dh.dtype != dtype or dh.device != device:
+        raise ValueError(f"dh must be a ({m}, {h}) {dtype} tensor on {device}")
+    index, size = device.index, 4 if kind == sdk.FP32 else 2
+    with torch.no_grad(), _on_device(index):
+        dh, lddh = _rows(dh)
+        dx = dh.new_empty((m, k)) if needs[0] else None
+        dwg = dh.new_empty((h, k)) if needs[1] else None
+        dwu = dh.new_empty((h, k)) if needs[2] else None
+        dbg = dh.new_empty((h,)) if needs[3] else None
+        dbu = dh.new_empty((h,)) if needs[4] else None
+        pg0 = pre.data_ptr()
+        d = Gated(_GATED_SIZE, kind, act, xt, wt, 0, m, h, k, x.data_ptr() + ox * size,
+                  w_gate.data_ptr() + og * size, w_up.data_ptr() + ou * size, ldx, ldg, ldu, 0, 0,
+                  pg0, pg0 + m * ldp * 4, ldp, 0, 0, _stream(index))
+        ws = _gated_workspace(d, 1, dh)  # noqa: F841  (alive until the launches)
+        _check(lib.xvram_b200_gated_backward(ctypes.byref(d), dh.data_ptr(), lddh, _ptr(dx), k,
+                                             _ptr(dwg), _ptr(dwu), k, _ptr(dbg), _ptr(dbu)),
                "xvram_b200_gated_backward")
-    return tuple(grads)
+    return dx, dwg, dwu, dbg, dbu
 
 
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
         out, saved = _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
-        ctx.save_for_backward(saved.x, saved.w_gate, saved.w_up, saved.pre_gate, saved.pre_up)
-        ctx.activation = activation
+        ctx.save_for_backward(*saved.tensors)
+        ctx.layout = saved.layout
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        saved = GatedSaved(*ctx.saved_tensors, ctx.activation)
-        return (*gated_linear_backward(dh, saved, ctx.needs_input_grad[:5]), None)
+        saved = GatedSaved(ctx.saved_tensors, ctx.layout)
+        return (*gated_linear_backward(dh, saved, ctx.needs_input_grad), None)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
@@ -329,10 +367,12 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     accumulation and one rounding, float32 in strict FP32.  Row-major and transposed operands
     are read in place (16-bit ones where their base and leading dimension are multiples of 16
     bytes; others are copied first).  Differentiable once in every tensor argument."""
-    tensors = (x, w_gate, w_up, bias_gate, bias_up)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _GatedLinear.apply(*tensors, activation)
-    return _gated_forward(*tensors, activation, False)[0]
+    if torch.is_grad_enabled() and (
+            x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
+            (bias_gate is not None and bias_gate.requires_grad) or
+            (bias_up is not None and bias_up.requires_grad)):
+        return _GatedLinear.apply(x, w_gate, w_up, bias_gate, bias_up, activation)
+    return _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, False)[0]
 
 
 @dataclasses.dataclass(frozen=True)
@@ -423,18 +463,19 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
     if dtype not in _FEED_TYPES or given not in _FEED_TYPES:
         raise TypeError(f"{what} supports float16, bfloat16 and float32 (got {given} to {dtype})")
     shape, device = x.shape, x.device
-    first = weights[0]
-    if len(shape) != 2 or any(not isinstance(w, Mxfp4Matrix) or w.shape[1] != shape[1] or
-                              w.shape[0] != first.shape[0] for w in weights):
+    first, last = weights[0], weights[-1]
+    if not isinstance(first, Mxfp4Matrix) or not isinstance(last, Mxfp4Matrix) or \
+            len(shape) != 2 or first.shape[1] != shape[1] or last.shape != first.shape:
         raise ValueError(f"{what} takes x (batch, in) and MXFP4 weights (out, in)")
     m, k = shape
     n = first.shape[0]
     if k == 0:
         raise ValueError(f"{what} needs at least one input feature")
-    if device.type != "cuda" or any(w.codes.device != device for w in weights):
+    if device.type != "cuda" or first.codes.device != device or last.codes.device != device:
         raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *biases)
-                                       if isinstance(t, torch.Tensor)):
+    if torch.is_grad_enabled() and (
+            (not quantised and x.requires_grad) or
+            any(b is not None and b.requires_grad for b in biases)):
         raise RuntimeError(f"{what} has no gradient: detach its input and biases")
     index = device.index
     with _on_device(index):
@@ -450,7 +491,6 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
             scales = codes + size
         out = like.new_empty((m, n), dtype=dtype)
         b = [None if t is None else _check_bias(t, n, dtype, device, "bias") for t in biases]
-        last = weights[-1]
         d = Mxfp4Product(_PRODUCT_SIZE, _FEED_TYPES[given], _FEED_TYPES[dtype], activation, m, n, k,
                          src, ldx, codes, scales, first.codes.data_ptr(), last.codes.data_ptr(),
                          first.scales.data_ptr(), last.scales.data_ptr(), _ptr(b[0]), _ptr(b[-1]),
