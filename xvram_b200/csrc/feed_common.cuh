@@ -274,7 +274,7 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// N (a multiple of 8) values of a row from column `col` on: 16-byte stores when the row allows
+// N (whole 16 bytes) values of a row from column `col` on: 16-byte stores when the row allows
 // them and all are inside n, else one by one.
 template <class T, int N>
 __device__ __forceinline__ void store_row(T* row, int col, int n, bool vec, const float (&v)[N]) {

@@ -67,6 +67,41 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t stage_bytes = scale_off + (K == Kind::mxf4 ? kScaleBytes : 0);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t sbase = smem_u32(smem);
+  const auto load_b = [&](int kt, int s) {
+    const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+    const int k0 = kt * kElems;
+    mbar_arrive_expect_tx(&full[s], stage_bytes);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : 0];
+      const int row = E == Epilogue::gated ? n0 : n0 + 128 * j;
+      const uint32_t d = base + b_off + j * kPart;
+      if (K == Kind::f16 && p.b_mn) {
+        tc::tma_load<1>(d, mb, bar, row, k0);
+        tc::tma_load<1>(d + kPart / 2, mb, bar, row + 64, k0);
+      } else {
+        tc::tma_load<1>(d, mb, bar, k0, row);
+      }
+      if constexpr (K == Kind::mxf4)
+        tc::tma_load<1>(base + scale_off + kScaleTile * (1 + j),
+                        &maps.scale_b[E == Epilogue::gated ? j : 0], bar, kt * 256,
+                        row / 128);
+    }
+  };
+  const auto load_a = [&](int kt, int s) {
+    const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+    const int k0 = kt * kElems;
+    if (K == Kind::f16 && p.a_mn) {
+      tc::tma_load<1>(base, &maps.a[0], bar, 0, k0);
+      tc::tma_load<1>(base + kPart / 2, &maps.a[0], bar, 64, k0);
+    } else {
+      tc::tma_load<1>(base, &maps.a[0], bar, k0, 0);
+    }
+    if constexpr (K == Kind::mxf4)
+      tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);
+  };
+  const int count = k_end - k_begin, ahead = min(count, q.stages);
   if (tid == 0) {
     for (int s = 0; s < q.stages; ++s) {
       mbar_init(&full[s], 1);
@@ -75,6 +110,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
+    // The producer's own barriers are ready: the first weights need not wait for the rest.
+    for (int i = 0; i < ahead; ++i)
+      load_b(k_begin + i, i);
   }
   if (warp == 1)
     tc::tmem_alloc<1>(tmem_slot, kTmemCols);
@@ -82,47 +120,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t sbase = smem_u32(smem);
 
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
-      const auto load_b = [&](int kt, int s) {
-        const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
-        const int k0 = kt * kElems;
-        mbar_arrive_expect_tx(&full[s], stage_bytes);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : 0];
-          const int row = E == Epilogue::gated ? n0 : n0 + 128 * j;
-          const uint32_t d = base + b_off + j * kPart;
-          if (K == Kind::f16 && p.b_mn) {
-            tc::tma_load<1>(d, mb, bar, row, k0);
-            tc::tma_load<1>(d + kPart / 2, mb, bar, row + 64, k0);
-          } else {
-            tc::tma_load<1>(d, mb, bar, k0, row);
-          }
-          if constexpr (K == Kind::mxf4)
-            tc::tma_load<1>(base + scale_off + kScaleTile * (1 + j),
-                            &maps.scale_b[E == Epilogue::gated ? j : 0], bar, kt * 256,
-                            row / 128);
-        }
-      };
-      const auto load_a = [&](int kt, int s) {
-        const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
-        const int k0 = kt * kElems;
-        if (K == Kind::f16 && p.a_mn) {
-          tc::tma_load<1>(base, &maps.a[0], bar, 0, k0);
-          tc::tma_load<1>(base + kPart / 2, &maps.a[0], bar, 64, k0);
-        } else {
-          tc::tma_load<1>(base, &maps.a[0], bar, k0, 0);
-        }
-        if constexpr (K == Kind::mxf4)
-          tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);
-      };
-      const int count = k_end - k_begin, ahead = min(count, q.stages);
-      for (int i = 0; i < ahead; ++i)
-        load_b(k_begin + i, i);
       asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < ahead; ++i)
         load_a(k_begin + i, i);
@@ -277,6 +278,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Rows of A that a stage holds.
 inline int split_rows(int m) { return std::min(128, (m + 7) / 8 * 8); }
 
+// CTAs of clusters of `size` (one CTA per SM) that the current device runs at once.
+template <class F>
+long long cluster_capacity(F* kernel, int size, long long sms) {
+  static std::atomic<int> known[64][4]; // by device and log2(size)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64)
+    return 0;
+  std::atomic<int>& slot = known[dev][size == 2 ? 1 : size == 4 ? 2 : 3];
+  int clusters = slot.load(std::memory_order_relaxed);
+  if (clusters == 0) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(sms / size * size));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSplitSmem;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
+      cudaGetLastError();
+      clusters = 0;
+    }
+    clusters = std::max(clusters, 0) + 1; // 0: not asked yet
+    slot.store(clusters, std::memory_order_relaxed);
+  }
+  return static_cast<long long>(clusters - 1) * size;
+}
+
 // `after`: launched behind a kernel of the same stream that allows programmatic overlap.
 template <Kind K, Epilogue E, class T>
 cudaError_t launch_split(const Maps& maps, const Params& p, bool after, cudaStream_t stream) {
@@ -290,15 +321,21 @@ cudaError_t launch_split(const Maps& maps, const Params& p, bool after, cudaStre
   q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
   const int stage = q.a_bytes + 2 * kPart + (K == Kind::mxf4 ? kScaleBytes : 0);
   q.stages = std::min(K == Kind::mxf4 ? 10 : kSplitMaxStages, kSplitRing / stage);
-  // A stage of all SMs takes about 0.75 us of HBM time; joining costs about 1 us and a little
-  // per CTA.  The split with the least of waves x stages, and joins, wins.
+  // Estimated time of a split, in us: a stage takes 0.75 when all SMs read from HBM and at least
+  // 0.45 (one SM's rate); a wave of CTAs 2.5 to start, joining 1.  Clusters fit an SM count that
+  // the hardware's grouping of SMs limits.
   const long long tiles = (p.n + kTileN - 1) / kTileN, sms = tc::sm_count();
   double best = 0;
   q.splits = 1;
   for (int s = 1; s <= 8 && s <= p.k_tiles; s *= 2) {
-    const double t = 0.75 * static_cast<double>((tiles * s + sms - 1) / sms) *
-                         ((p.k_tiles + s - 1) / s) +
-                     (s > 1 ? 1.0 + 0.1 * s : 0.0);
+    const long long ctas = tiles * s, cap = s == 1 ? sms : cluster_capacity(kernel, s, sms);
+    if (cap < s)
+      break;
+    const double stage_us =
+        std::max(0.45, 0.75 * static_cast<double>(std::min(ctas, cap)) / static_cast<double>(sms));
+    const double t = static_cast<double>((ctas + cap - 1) / cap) *
+                         (2.5 + stage_us * ((p.k_tiles + s - 1) / s)) +
+                     (s > 1 ? 1.0 : 0.0);
     if (s == 1 || t < best) {
       best = t;
       q.splits = s;

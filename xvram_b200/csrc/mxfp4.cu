@@ -16,7 +16,10 @@
 #include "feed_split.cuh"
 #include "kernels.hpp"
 
+#include <cuda_fp4.h>
+
 #include <algorithm>
+#include <cstring>
 
 namespace xvram {
 
@@ -28,19 +31,15 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 constexpr int kBlock = 32;
 
-// Eight floats to eight E2M1 codes, the first in the lowest four bits.
-__device__ __forceinline__ uint32_t to_e2m1(const float (&v)[8]) {
-  uint32_t r;
-  asm("{\n"
-      "  .reg .b8 b0, b1, b2, b3;\n"
-      "  cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n"
-      "  cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
-      "  cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n"
-      "  cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
-      "  mov.b32 %0, {b0, b1, b2, b3};\n"
-      "}\n"
-      : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+// Eight floats from v[FROM] on to eight E2M1 codes, the first in the lowest four bits.
+template <int FROM>
+__device__ __forceinline__ uint32_t to_e2m1(const float (&v)[16]) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(
+             make_float2(v[FROM + 2 * i], v[FROM + 2 * i + 1]), __NV_E2M1, cudaRoundNearest))
+         << (8 * i);
   return r;
 }
 
@@ -50,24 +49,42 @@ __device__ __forceinline__ float scale_value(uint32_t s) {
                   : __uint_as_float(s ? s << 23 : 0x00400000u);
 }
 
-// Values v[0..8) from column c of a row; zeros past the end.
-template <class T>
-__device__ __forceinline__ void load8(const T* row, long long c, int cols, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= cols) {
-    alignas(16) T t[8];
-    if constexpr (sizeof(T) == 2) {
-      *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(row + c);
-    } else {
-      reinterpret_cast<uint4*>(t)[0] = *reinterpret_cast<const uint4*>(row + c);
-      reinterpret_cast<uint4*>(t)[1] = *reinterpret_cast<const uint4*>(row + c + 4);
-    }
+// The largest magnitude (as float bits) by its bits, which order NaN above infinity above finite
+// values.
+__device__ __forceinline__ uint32_t top_of(const float (&t)[16]) {
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = to_float(t[i]);
+  for (int i = 0; i < 16; ++i)
+    top = max(top, __float_as_uint(t[i]) & 0x7fffffffu);
+  return top;
+}
+template <class T>
+__device__ __forceinline__ uint32_t top_of(const T (&t)[16]) { // two 16-bit values at a time
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(t);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+  const unsigned short m = static_cast<unsigned short>(max(top >> 16, top & 0xffffu));
+  T v;
+  memcpy(&v, &m, 2);
+  return __float_as_uint(to_float(v));
+}
+template <class T>
+struct Values16 {
+  alignas(16) T t[16];
+};
+template <class T>
+__device__ __forceinline__ void load16(const T* row, long long c, int cols, bool vec,
+                                       Values16<T>& v) {
+  if (vec && c + 16 <= cols) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i)
+      reinterpret_cast<uint4*>(v.t)[i] = reinterpret_cast<const uint4*>(row + c)[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
+    for (int i = 0; i < 16; ++i)
+      v.t[i] = c + i < cols ? row[c + i] : from_float<T>(0.0f);
   }
 }
 
@@ -76,70 +93,121 @@ __device__ __forceinline__ size_t scale_index(long long r, int b, int block_tile
          ((r >> 5) & 3) * 4 + (b & 3);
 }
 
-// Four lanes to a block, eight values each.  HBM-bound: the values in, 17 bytes out per block.
+// Both passes: blocks of 256 threads as 256 / tx rows of tx threads, `units` threads to a row,
+// each for `each` rows: enough bytes in flight per thread that HBM, and not the blocks'
+// latency, bounds large matrices, and one row where there are few blocks.
+struct PassGrid {
+  int tx, each;
+  dim3 grid;
+};
+PassGrid pass_grid(long long rows, int units, int most) {
+  PassGrid g;
+  g.tx = 8;
+  while (g.tx < units && g.tx < 256)
+    g.tx *= 2;
+  const long long across = (units + g.tx - 1) / g.tx;
+  long long per = 256 / g.tx;
+  const bool many = across * ((rows + per - 1) / per) >= 16ll * tc::sm_count();
+  g.each = many ? most : 1;
+  per *= g.each;
+  g.grid = dim3(static_cast<unsigned>(across),
+                static_cast<unsigned>(std::min((rows + per - 1) / per, 65535ll)));
+  return g;
+}
+
+// Two lanes to a block, 16 values each: fewer instructions per value than with smaller shares.
 // The grid covers the scales' padded rows and blocks, whose bytes it sets to 127.  A product
 // launched behind it with programmatic overlap may start loading its weights at once.
-template <class T>
+constexpr int kQuantizeRows = 2;
+template <class T, int EACH>
 __global__ void __launch_bounds__(256)
     mxfp4_quantize_kernel(const T* __restrict__ src, long long lds, bool vec, int rows, int cols,
                           int blocks, int block_tiles, unsigned char* __restrict__ codes,
-                          unsigned char* __restrict__ scales, long long units) {
+                          unsigned char* __restrict__ scales, int tx) {
   asm volatile("griddepcontrol.launch_dependents;");
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < units; i += gridDim.x * 256ll) {
-    const int sub = static_cast<int>(i & 3);
-    const long long r = (i >> 2) / (4 * block_tiles);
-    const int b = static_cast<int>((i >> 2) - r * (4 * block_tiles));
-    const bool inside = r < rows && b < blocks;
-    float v[8] = {};
-    if (inside)
-      load8(src + r * lds, static_cast<long long>(b) * kBlock + sub * 8, cols, vec, v);
-    // The largest magnitude by its bits, which order NaN above infinity above finite values.
-    uint32_t top = 0;
+  const int unit = blockIdx.x * tx + (threadIdx.x & (tx - 1));
+  const int b = unit >> 1, sub = unit & 1, step = 256 / tx;
+  const long long padded = (rows + 127ll) / 128 * 128;
+  const unsigned peers = 0xffu << (threadIdx.x & 24);
+  if (b >= 4 * block_tiles)
+    return; // whole groups of 8 lanes
+  for (long long r0 = static_cast<long long>(blockIdx.y) * (step * EACH) + threadIdx.x / tx;
+       r0 < padded; r0 += static_cast<long long>(gridDim.y) * (step * EACH)) {
+    Values16<T> raw[EACH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-    const unsigned peers = 0xfu << (threadIdx.x & 28);
-    top = max(top, __shfl_xor_sync(peers, top, 1));
-    top = max(top, __shfl_xor_sync(peers, top, 2));
-    const int e = static_cast<int>(top >> 23); // floor(log2) + 127 of a normal value
-    const uint32_t s = e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
-    if (inside) {
-      uint32_t code = 0;
-      if (s != 255) {
-        const float inv = __uint_as_float((254u - s) << 23); // 2^(127 - s)
+    for (int j = 0; j < EACH; ++j)
+      if (r0 + j * step < rows && b < blocks)
+        load16(src + (r0 + j * step) * lds, static_cast<long long>(b) * kBlock + sub * 16, cols, vec,
+               raw[j]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          v[j] *= inv;
-        code = to_e2m1(v);
+    for (int j = 0; j < EACH; ++j) {
+      const long long r = r0 + j * step;
+      const bool inside = r < rows && b < blocks;
+      uint32_t top = inside ? top_of(raw[j].t) : 0;
+      top = max(top, __shfl_xor_sync(peers, top, 1));
+      const int e = static_cast<int>(top >> 23); // floor(log2) + 127 of a normal value
+      uint32_t s = e == 255 ? 255u : static_cast<uint32_t>(max(e - 2, 0));
+      if (inside) {
+        const float inv = __uint_as_float((254u - min(s, 254u)) << 23); // 2^(127 - s)
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[i] = to_float(raw[j].t[i]) * inv;
+        uint2 code = make_uint2(to_e2m1<0>(v), to_e2m1<8>(v));
+        if (s == 255)
+          code = make_uint2(0, 0);
+        reinterpret_cast<uint2*>(codes)[(r * blocks + b) * 2 + sub] = code;
+      } else {
+        s = 127;
       }
-      reinterpret_cast<uint32_t*>(codes)[(r * blocks + b) * 4 + sub] = code;
+      // Four blocks' scales are neighbouring bytes.
+      s |= __shfl_down_sync(peers, s, 2, 8) << 8;
+      s |= __shfl_down_sync(peers, s, 4, 8) << 16;
+      if ((threadIdx.x & 7) == 0 && r < padded)
+        *reinterpret_cast<uint32_t*>(scales + scale_index(r, b, block_tiles)) = s;
     }
-    if (sub == 0)
-      scales[scale_index(r, b, block_tiles)] = static_cast<unsigned char>(inside ? s : 127u);
   }
 }
 
-template <class T>
+// 16 bytes of results per thread and row.
+constexpr int kDequantizeRows = 8;
+template <class T, int EACH>
 __global__ void __launch_bounds__(256)
     mxfp4_dequantize_kernel(const unsigned char* __restrict__ codes,
-                            const unsigned char* __restrict__ scales, int cols, int blocks,
-                            int block_tiles, T* __restrict__ dst, long long ldd, bool vec,
-                            long long units) {
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < units; i += gridDim.x * 256ll) {
-    const int sub = static_cast<int>(i & 3);
-    const long long r = (i >> 2) / blocks;
-    const int b = static_cast<int>((i >> 2) - r * blocks);
-    const uint32_t code = reinterpret_cast<const uint32_t*>(codes)[i];
-    const float x = scale_value(scales[scale_index(r, b, block_tiles)]);
-    float v[8];
+                            const unsigned char* __restrict__ scales, int rows, int cols,
+                            int blocks, int block_tiles, T* __restrict__ dst, long long ldd,
+                            bool vec, int tx) {
+  constexpr int per = 16 / sizeof(T), lanes = kBlock / per; // values per thread, threads per block
+  const int unit = blockIdx.x * tx + (threadIdx.x & (tx - 1));
+  const int b = unit / lanes, sub = unit % lanes, step = 256 / tx;
+  if (b >= blocks)
+    return;
+  for (long long r0 = static_cast<long long>(blockIdx.y) * (step * EACH) + threadIdx.x / tx;
+       r0 < rows; r0 += static_cast<long long>(gridDim.y) * (step * EACH)) {
+    uint32_t code[EACH], scale[EACH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // The three magnitude bits as the low exponent bits and the top mantissa bit of a float:
-      // E2M1 * 2^-126, subnormals included; times 2^126 exactly.
-      const uint32_t c = code >> (4 * j);
-      v[j] = __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28)) * 0x1p126f * x;
+    for (int j = 0; j < EACH; ++j) {
+      const long long r = min(r0 + j * step, rows - 1ll);
+      const unsigned char* c = codes + (r * blocks + b) * 16 + sub * (per / 2);
+      code[j] = per == 8 ? *reinterpret_cast<const uint32_t*>(c)
+                         : *reinterpret_cast<const unsigned short*>(c);
+      scale[j] = scales[scale_index(r, b, block_tiles)];
     }
-    store_row(dst + r * ldd, b * kBlock + sub * 8, cols, vec, v);
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const long long r = r0 + j * step;
+      const float f = scale_value(scale[j]);
+      float v[per];
+#pragma unroll
+      for (int i = 0; i < per; ++i) {
+        // The three magnitude bits as the low exponent bits and the top mantissa bit of a
+        // float: E2M1 * 2^-126, subnormals included; times 2^126 exactly.
+        const uint32_t t = code[j] >> (4 * i);
+        v[i] = __uint_as_float(((t & 7u) << 22) | ((t & 8u) << 28)) * 0x1p126f * f;
+      }
+      if (r < rows)
+        store_row(dst + r * ldd, b * kBlock + sub * per, cols, vec, v);
+    }
   }
 }
 
@@ -148,19 +216,15 @@ bool vec_rows(const void* p, long long ld) {
   return aligned16(p) && ld % static_cast<long long>(16 / sizeof(T)) == 0;
 }
 
-unsigned blocks_for(long long units) {
-  return static_cast<unsigned>(
-      std::max<long long>(1, std::min<long long>((units + 255) / 256, 16ll * tc::sm_count())));
-}
-
 template <class T>
 cudaError_t quantize(const void* src, long long lds, int rows, int cols, unsigned char* codes,
                      unsigned char* scales, cudaStream_t stream) {
   const int blocks = (cols + kBlock - 1) / kBlock, tiles = (blocks + 3) / 4;
-  const long long units = ((rows + 127ll) / 128 * 128) * tiles * 16ll;
-  mxfp4_quantize_kernel<T><<<blocks_for(units), 256, 0, stream>>>(
-      static_cast<const T*>(src), lds, vec_rows<T>(src, lds), rows, cols, blocks, tiles, codes,
-      scales, units);
+  const PassGrid g = pass_grid((rows + 127ll) / 128 * 128, tiles * 8, kQuantizeRows);
+  const auto kernel =
+      g.each > 1 ? mxfp4_quantize_kernel<T, kQuantizeRows> : mxfp4_quantize_kernel<T, 1>;
+  kernel<<<g.grid, 256, 0, stream>>>(static_cast<const T*>(src), lds, vec_rows<T>(src, lds), rows,
+                                     cols, blocks, tiles, codes, scales, g.tx);
   return cudaGetLastError();
 }
 
@@ -168,9 +232,12 @@ template <class T>
 cudaError_t dequantize(const unsigned char* codes, const unsigned char* scales, int rows, int cols,
                        void* dst, long long ldd, cudaStream_t stream) {
   const int blocks = (cols + kBlock - 1) / kBlock, tiles = (blocks + 3) / 4;
-  const long long units = static_cast<long long>(rows) * blocks * 4;
-  mxfp4_dequantize_kernel<T><<<blocks_for(units), 256, 0, stream>>>(
-      codes, scales, cols, blocks, tiles, static_cast<T*>(dst), ldd, vec_rows<T>(dst, ldd), units);
+  const PassGrid g =
+      pass_grid(rows, blocks * (kBlock * static_cast<int>(sizeof(T)) / 16), kDequantizeRows);
+  const auto kernel =
+      g.each > 1 ? mxfp4_dequantize_kernel<T, kDequantizeRows> : mxfp4_dequantize_kernel<T, 1>;
+  kernel<<<g.grid, 256, 0, stream>>>(codes, scales, rows, cols, blocks, tiles,
+                                     static_cast<T*>(dst), ldd, vec_rows<T>(dst, ldd), g.tx);
   return cudaGetLastError();
 }
 
