@@ -410,13 +410,13 @@ cudaError_t forward_rows(const GatedProblem& q, void* out, long long ldo, cudaSt
 //   548 us for the FFMA kernel, whose waves of 148 128 x 128 tiles take 0.066 us per input whatever
 //   m is; 1024 x 2048: 62 us for 128 rows against 136.  4 m h k / 20 TFLOP/s is below the two GEMMs'
 //   2 x 0.066 us k waves while m h < 640k waves.
-//   BF16, same sizes: 25 and 3.9 us for one row, 34 and 5.0 for 4, 64 and 6.3 for 8, against the
-//   tensor cores' 35-40 and 11.
+//   BF16: 4096 x 8192 25 us for one row, 34 for 4, against the tensor cores' 26; 1024 x 2048 4.2 us for
+//   one row and 4.9 for 4, against 7.
 bool few_rows(const GatedProblem& q) {
   if (q.x_transposed || q.w_transposed)
     return false;
   if (q.type != GatedType::f32)
-    return q.m <= 4;
+    return q.m == 1 || (q.m <= 4 && static_cast<long long>(q.h) * q.k <= 8 << 20);
   if (q.m > 512)
     return false;
   const long long tiles = ((q.h + 127ll) / 128) * ((q.m + 127) / 128), sms = tc::sm_count();

@@ -39,8 +39,6 @@ import contextlib
 import ctypes
 import threading
 
-import dataclasses
-
 import torch
 
 from . import device as xd
@@ -375,29 +373,27 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     return _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, False)[0]
 
 
-@dataclasses.dataclass(frozen=True)
 class Mxfp4Matrix:
     """A (rows, cols) matrix in microscaled 4-bit floating point, stored as
     include/xvram_b200.h lays it out: `codes` rows x ceil(cols / 32) x 16 bytes, `scales`
     ceil(rows / 128) x ceil(cols / 128) tiles of 512 bytes, both contiguous uint8 CUDA tensors of
     any shape.  Codes past the last column must be 0 and scales past the end not 255."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    shape: tuple[int, int]
+    __slots__ = ("codes", "scales", "shape")
 
-    def __post_init__(self):
-        rows, cols = self.shape
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int]):
+        rows, cols = shape
         if rows < 0 or cols < 0:
             raise ValueError("negative size")
-        for t, need, name in ((self.codes, rows * ((cols + 31) // 32) * 16, "codes"),
-                              (self.scales, ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
+        for t, need, name in ((codes, rows * ((cols + 31) // 32) * 16, "codes"),
+                              (scales, ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
                                "scales")):
             if t.dtype != torch.uint8 or t.numel() != need or not t.is_contiguous() or \
                     t.data_ptr() % 16:
                 raise ValueError(f"{name} of a ({rows}, {cols}) MXFP4 matrix must be {need} "
                                  "contiguous bytes (uint8), 16-byte aligned")
-        if self.codes.device != self.scales.device:
+        if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
+        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
 
     @property
     def device(self) -> torch.device:
@@ -435,7 +431,9 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
                                              codes.data_ptr(), scales.data_ptr(),
                                              _stream(x.device.index)),
                "xvram_b200_mxfp4_quantize")
-    return Mxfp4Matrix(codes, scales, (rows, cols))
+    q = Mxfp4Matrix.__new__(Mxfp4Matrix)  # its invariants hold: no checks
+    q.codes, q.scales, q.shape = codes, scales, (rows, cols)
+    return q
 
 
 def dequantize_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.float32) -> torch.Tensor:
