@@ -9,6 +9,8 @@
 
 #include "feed_common.cuh"
 
+#include <type_traits>
+
 namespace xvram::feed {
 
 struct RowsParams {
@@ -22,107 +24,117 @@ struct RowsParams {
   int m, h, k, act;
 };
 
-template <class T>
-struct Vec16 { // 16 bytes of values
-  static constexpr int n = 16 / sizeof(T);
-  alignas(16) T v[n];
+template <class T, int N>
+struct Values {
+  alignas(N * sizeof(T)) T v[N];
 };
 
-template <class T>
-__device__ __forceinline__ void load_stream(const T* p, Vec16<T>& d) {
-  uint4 t;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
-               : "l"(p));
-  *reinterpret_cast<uint4*>(d.v) = t;
+// Weights: read once, so not kept in L1.  Volatile, so that a block's loads stay together ahead of
+// the arithmetic.
+template <class T, int N>
+__device__ __forceinline__ void load_stream(const T* p, Values<T, N>& d) {
+  if constexpr (N * sizeof(T) == 16) {
+    uint4 t;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
+                 : "l"(p));
+    *reinterpret_cast<uint4*>(d.v) = t;
+  } else if constexpr (sizeof(T) == 4) {
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(d.v[0]) : "l"(p));
+  } else {
+    unsigned short t;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(t) : "l"(p));
+    *reinterpret_cast<unsigned short*>(d.v) = t;
+  }
 }
 
 // VEC: values a lane reads at once (16 bytes' worth, or 1 when rows are not 16-byte aligned).
 template <class T, int MR, int HPW, int VEC>
-__global__ void __launch_bounds__(256) feed_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(256, 2) feed_rows_kernel(const RowsParams p) {
   constexpr int NV = 2 * HPW * MR;
   static_assert((NV & (NV - 1)) == 0 && NV <= 32, "sums are a power of two");
-  constexpr int UNROLL = VEC == 1 || NV < 16 ? 4 : 2;
+  constexpr int UNROLL = 4;
   __shared__ float sums[8][NV];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long h0 = (blockIdx.x * 8ll + warp) * HPW;
   const int r0 = blockIdx.y * MR;
   if (h0 >= p.h)
     return; // whole warps
-  const T* x = static_cast<const T*>(p.x) + r0 * p.ldx;
-  const T *wg[HPW], *wu[HPW];
+  const T *x[MR], *wg[HPW], *wu[HPW];
 #pragma unroll
   for (int i = 0; i < HPW; ++i) { // rows past the end repeat the last one
     const long long h = min(h0 + i, static_cast<long long>(p.h) - 1);
-    wg[i] = static_cast<const T*>(p.w_gate) + h * p.ld_gate;
-    wu[i] = static_cast<const T*>(p.w_up) + h * p.ld_up;
+    wg[i] = static_cast<const T*>(p.w_gate) + h * p.ld_gate + lane * VEC;
+    wu[i] = static_cast<const T*>(p.w_up) + h * p.ld_up + lane * VEC;
   }
-  long long xo[MR];
 #pragma unroll
   for (int r = 0; r < MR; ++r)
-    xo[r] = min(r, p.m - 1 - r0) * p.ldx;
+    x[r] = static_cast<const T*>(p.x) + min(r0 + r, p.m - 1) * p.ldx + lane * VEC;
 
   float acc[NV] = {}; // [row][output][gate, up]
-  const auto step = [&](int k) {
-    if constexpr (VEC == 1) {
-      float g[HPW], u[HPW];
+  const auto block = [&](auto count) { // `count` steps from the pointers on
+    constexpr int U = decltype(count)::value;
+    Values<T, VEC> g[U][HPW], u[U][HPW];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
 #pragma unroll
       for (int i = 0; i < HPW; ++i) {
-        g[i] = to_float(wg[i][k]);
-        u[i] = to_float(wu[i][k]);
+        load_stream(wg[i] + j * 32 * VEC, g[j][i]);
+        load_stream(wu[i] + j * 32 * VEC, u[j][i]);
       }
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
 #pragma unroll
       for (int r = 0; r < MR; ++r) {
-        const float xv = to_float(x[xo[r] + k]);
+        const Values<T, VEC> xv =
+            *reinterpret_cast<const Values<T, VEC>*>(x[r] + j * 32 * VEC);
 #pragma unroll
-        for (int i = 0; i < HPW; ++i) {
-          acc[(r * HPW + i) * 2] = fmaf(xv, g[i], acc[(r * HPW + i) * 2]);
-          acc[(r * HPW + i) * 2 + 1] = fmaf(xv, u[i], acc[(r * HPW + i) * 2 + 1]);
-        }
-      }
-    } else {
-      Vec16<T> g[HPW], u[HPW];
-#pragma unroll
-      for (int i = 0; i < HPW; ++i) {
-        load_stream(wg[i] + k, g[i]);
-        load_stream(wu[i] + k, u[i]);
-      }
-#pragma unroll
-      for (int r = 0; r < MR; ++r) {
-        Vec16<T> xv;
-        *reinterpret_cast<uint4*>(xv.v) = *reinterpret_cast<const uint4*>(x + xo[r] + k);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float f = to_float(xv.v[j]);
+        for (int e = 0; e < VEC; ++e) {
+          const float f = to_float(xv.v[e]);
 #pragma unroll
           for (int i = 0; i < HPW; ++i) {
-            acc[(r * HPW + i) * 2] = fmaf(f, to_float(g[i].v[j]), acc[(r * HPW + i) * 2]);
-            acc[(r * HPW + i) * 2 + 1] = fmaf(f, to_float(u[i].v[j]), acc[(r * HPW + i) * 2 + 1]);
+            float* a = acc + (r * HPW + i) * 2;
+            a[0] = fmaf(f, to_float(g[j][i].v[e]), a[0]);
+            a[1] = fmaf(f, to_float(u[j][i].v[e]), a[1]);
           }
         }
       }
     }
   };
+  // The pointers advance, so that the loads of an unrolled step differ by constants alone.
   constexpr int kStride = 32 * VEC;
-  int k = lane * VEC;
-  for (; k + (UNROLL - 1) * kStride + VEC <= p.k; k += UNROLL * kStride) {
+  const auto advance = [&](int by) {
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j)
-      step(k + j * kStride);
+    for (int i = 0; i < HPW; ++i) {
+      wg[i] += by;
+      wu[i] += by;
+    }
+#pragma unroll
+    for (int r = 0; r < MR; ++r)
+      x[r] += by;
+  };
+  int left = p.k - lane * VEC; // values from the pointers to the end
+  for (; left >= (UNROLL - 1) * kStride + VEC; left -= UNROLL * kStride) {
+    block(std::integral_constant<int, UNROLL>{});
+    advance(UNROLL * kStride);
   }
-  for (; k + VEC <= p.k; k += kStride)
-    step(k);
-  // 16-byte rows whose length is not whole 16 bytes: the last k % VEC values, one per lane.
+  for (; left >= VEC; left -= kStride) {
+    block(std::integral_constant<int, 1>{});
+    advance(kStride);
+  }
+  // 16-byte rows whose length is not whole 16 bytes: the lane whose values end the row.
   if constexpr (VEC > 1) {
-    const int t = p.k / VEC * VEC + lane;
-    if (t < p.k) {
+    if (left > 0) {
+      for (int t = 0; t < left; ++t) {
 #pragma unroll
-      for (int r = 0; r < MR; ++r) {
-        const float f = to_float(x[xo[r] + t]);
+        for (int r = 0; r < MR; ++r) {
+          const float f = to_float(x[r][t]);
 #pragma unroll
-        for (int i = 0; i < HPW; ++i) {
-          acc[(r * HPW + i) * 2] = fmaf(f, to_float(wg[i][t]), acc[(r * HPW + i) * 2]);
-          acc[(r * HPW + i) * 2 + 1] = fmaf(f, to_float(wu[i][t]), acc[(r * HPW + i) * 2 + 1]);
+          for (int i = 0; i < HPW; ++i) {
+            acc[(r * HPW + i) * 2] = fmaf(f, to_float(wg[i][t]), acc[(r * HPW + i) * 2]);
+            acc[(r * HPW + i) * 2 + 1] = fmaf(f, to_float(wu[i][t]), acc[(r * HPW + i) * 2 + 1]);
+          }
         }
       }
     }
