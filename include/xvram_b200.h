@@ -476,9 +476,13 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
  *   gated:  out (m x n) = act(x W0^T + bias[0]) * (x W1^T + bias[1]).
  * x (m x k): with x set, rows of `x_type` values, ldx elements apart, which are quantised into
  * x_codes and x_scales first (caller's memory, as xvram_b200_mxfp4_bytes says; it may be reused
- * once the call's work on `stream` is done); with x = 0, x_codes and x_scales as they are.  Biases
- * (0 for none) hold n values of out_type.
+ * once the call's work on `stream` is done); up to XVRAM_B200_MXFP4_DIRECT_ROWS rows of at most
+ * XVRAM_B200_MXFP4_DIRECT_VALUES values together are quantised inside the product instead, and
+ * x_codes and x_scales are not used (0 allowed).  With x = 0, x_codes and x_scales as they are.  Biases (0 for
+ * none) hold n values of out_type.
  */
+#define XVRAM_B200_MXFP4_DIRECT_ROWS 16
+#define XVRAM_B200_MXFP4_DIRECT_VALUES 65536
 typedef struct xvram_b200_mxfp4_product_v1 {
   uint32_t struct_size; /* sizeof(xvram_b200_mxfp4_product_v1) */
   uint32_t x_type, out_type; /* XVRAM_DATA_FP16, _BF16 or _FP32 */

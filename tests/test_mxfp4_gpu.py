@@ -125,7 +125,11 @@ def test_quantisation_of_strided_rows():
 
 
 SHAPES = [(1, 1, 1), (1, 8, 32), (3, 5, 7), (16, 128, 64), (128, 256, 256), (129, 257, 300),
-          (130, 130, 96), (40, 700, 1000), (257, 384, 2080)]
+          (130, 130, 96), (40, 700, 1000), (257, 384, 2080),
+          # Up to 16 rows and 65536 values are quantised inside the product: the most rows, one row
+          # and one value more, the longest rows.
+          (16, 3000, 4096), (16, 300, 4097), (17, 260, 2100), (1, 130, 65536), (1, 64, 65568),
+          (8, 130, 8192)]
 
 
 def operands(kind, m, n, k, seed, count):

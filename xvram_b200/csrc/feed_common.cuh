@@ -130,13 +130,14 @@ __device__ __forceinline__ void stage_f16(const Params& p, uint32_t d, uint32_t 
 // (the stage's barrier says so).  K past the end has zero codes and zero (2^-127) scales.
 template <int PAIR>
 __device__ __forceinline__ void stage_mxf4(const Params& p, uint32_t d, uint32_t a, uint32_t b,
-                                           uint32_t scales, uint32_t sf, bool first) {
+                                           uint32_t scale_a, uint32_t scale_b, uint32_t sf,
+                                           bool first) {
   const uint32_t sfa = sf, sfb = sf + 8;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
-    copy_scales<PAIR>(sfa + 4 * g, scales + 512 * g);
-    copy_scales<PAIR>(sfb + 8 * g, scales + kScaleTile + 512 * g);
-    copy_scales<PAIR>(sfb + 8 * g + 4, scales + 2 * kScaleTile + 512 * g);
+    copy_scales<PAIR>(sfa + 4 * g, scale_a + 512 * g);
+    copy_scales<PAIR>(sfb + 8 * g, scale_b + 512 * g);
+    copy_scales<PAIR>(sfb + 8 * g + 4, scale_b + kScaleTile + 512 * g);
   }
   const uint64_t da = tc::desc_kmajor(a), db = tc::desc_kmajor(b);
 #pragma unroll

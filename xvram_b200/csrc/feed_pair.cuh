@@ -183,8 +183,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if constexpr (K == Kind::f16)
           stage_f16<2>(p, d, a, b, first_k);
         else
-          stage_mxf4<2>(p, d, a, b, base + Shape::kScales, tmem + kScaleCol + stage * kScaleCols,
-                        first_k);
+          stage_mxf4<2>(p, d, a, b, base + Shape::kScales, base + Shape::kScales + kScaleTile,
+                        tmem + kScaleCol + stage * kScaleCols, first_k);
       };
       const auto next = [&] {
         if (++s == kPairStages) {

@@ -14,20 +14,36 @@
 //   warp 0      one lane: TMA loads; weights first, A once the preceding kernel (the
 //               quantisation of A, launched with programmatic overlap) is complete;
 //   warp 1      one lane: issues the MMAs;
-//   warps 2..9  empty the accumulator into shared memory; then all warps reduce and finish.
+//   warps 2..9  (MXFP4, few rows) quantise the CTA's K range of A into shared memory, in the
+//               layout a TMA load would leave, under the first weights' loads;
+//               empty the accumulator into shared memory; then all warps reduce and finish.
 #pragma once
 
-#include "feed_common.cuh"
+#include "mxfp4_block.cuh"
 
 #include <algorithm>
 
 namespace xvram::feed {
 
+// MXFP4: A as the caller's floats, quantised by the kernel (x = 0: A comes from the maps).
+constexpr int kDirectRows = 16;
+constexpr int kDirectValues = 65536; // rows x values
+constexpr int kDirectBytes = 96 * 1024; // shared memory of a CTA's quantised A, at most
+struct DirectInput {
+  const void* x;
+  long long ldx;
+  int type; // 0 FP16, 1 BF16, 2 FP32
+  int vec;  // 16-byte loads
+  int blocks, k;
+};
+
 struct SplitParams {
   Params p;
+  DirectInput in;
   int splits;      // cluster size
   int stages;      // ring depth
   int a_bytes;     // A's bytes per stage
+  int ring;        // offset of the stage ring (behind a quantised A)
 };
 
 constexpr int kSplitSmem = 222 * 1024;
@@ -44,6 +60,47 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
   return v;
 }
 
+// Blocks [first, last) of rows 0..m of x, two lanes to a block, to the stages' A tiles (codes,
+// 128-byte swizzle) and scale tiles; blocks past the end are zeros with scale 127.
+template <class X>
+__device__ __forceinline__ void quantize_rows(const DirectInput& in, int m, int first, int last,
+                                              unsigned char* codes, int a_bytes,
+                                              unsigned char* scales, int thread, int threads) {
+  constexpr int kEach = 4; // half blocks per thread and turn, loaded before the first is used
+  const X* x = static_cast<const X*>(in.x);
+  const int width = 2 * (last - first), units = m * width; // width: a multiple of 16
+  const unsigned peers = 3u << (threadIdx.x & 30);
+  for (int u0 = thread; u0 < units; u0 += kEach * threads) { // whole groups of 16 lanes
+    Values16<X> v[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int u = u0 + j * threads, r = u / width, i = u - r * width;
+      if (u < units && first + (i >> 1) < in.blocks)
+        load16(x + r * in.ldx, static_cast<long long>(first + (i >> 1)) * kBlock + (i & 1) * 16,
+               in.k, in.vec != 0, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int u = u0 + j * threads;
+      if (u >= units)
+        break;
+      const int r = u / width, i = u - r * width;
+      const int local = i >> 1, sub = i & 1;
+      const bool inside = first + local < in.blocks;
+      uint32_t top = inside ? top_of(v[j].t) : 0;
+      top = max(top, __shfl_xor_sync(peers, top, 1));
+      const uint32_t s = inside ? scale_byte(top) : 127u;
+      const uint2 code = inside ? codes16(v[j], s) : make_uint2(0, 0);
+      const int stage = local >> 3, chunk = local & 7;
+      *reinterpret_cast<uint2*>(codes + stage * a_bytes + r * 128 + ((chunk ^ (r & 7)) * 16) +
+                                sub * 8) = code;
+      if (sub == 0)
+        scales[stage * kScaleTile + (chunk >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 +
+               (chunk & 3)] = static_cast<unsigned char>(s);
+    }
+  }
+}
+
 template <Kind K, Epilogue E, class T>
 __global__ void __launch_bounds__(kThreads, 1)
     feed_split_kernel(const __grid_constant__ Maps maps, const SplitParams q) {
@@ -56,20 +113,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kSplitRing);
   uint64_t* empty = full + kSplitMaxStages;
   uint64_t* acc_full = empty + kSplitMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* a_ready = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(a_ready + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int rank = q.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
   const int n0 = static_cast<int>(blockIdx.x / q.splits) * kTileN;
   const int k_begin = static_cast<int>(static_cast<long long>(p.k_tiles) * rank / q.splits);
   const int k_end = static_cast<int>(static_cast<long long>(p.k_tiles) * (rank + 1) / q.splits);
-  const uint32_t b_off = q.a_bytes, scale_off = b_off + 2 * kPart;
-  const uint32_t stage_bytes = scale_off + (K == Kind::mxf4 ? kScaleBytes : 0);
+  const bool direct = K == Kind::mxf4 && q.in.x;
+  const int count = k_end - k_begin, ahead = min(count, q.stages);
+  // A stage: A, both parts of B, A's scales, B's scales; a quantised A lies in front of the ring.
+  const uint32_t b_off = direct ? 0 : q.a_bytes, scale_off = b_off + 2 * kPart;
+  const uint32_t scale_b_off = scale_off + (direct ? 0 : kScaleTile);
+  const uint32_t stage_bytes = K == Kind::mxf4 ? scale_b_off + 2 * kScaleTile : scale_off;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t sbase = smem_u32(smem);
+  const uint32_t sbase = smem_u32(smem), ring = sbase + q.ring;
   const auto load_b = [&](int kt, int s) {
-    const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+    const uint32_t bar = smem_u32(&full[s]), base = ring + s * stage_bytes;
     const int k0 = kt * kElems;
     mbar_arrive_expect_tx(&full[s], stage_bytes);
 #pragma unroll
@@ -84,13 +146,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tma_load<1>(d, mb, bar, k0, row);
       }
       if constexpr (K == Kind::mxf4)
-        tc::tma_load<1>(base + scale_off + kScaleTile * (1 + j),
+        tc::tma_load<1>(base + scale_b_off + kScaleTile * j,
                         &maps.scale_b[E == Epilogue::gated ? j : 0], bar, kt * 256,
                         row / 128);
     }
   };
   const auto load_a = [&](int kt, int s) {
-    const uint32_t bar = smem_u32(&full[s]), base = sbase + s * stage_bytes;
+    const uint32_t bar = smem_u32(&full[s]), base = ring + s * stage_bytes;
     const int k0 = kt * kElems;
     if (K == Kind::f16 && p.a_mn) {
       tc::tma_load<1>(base, &maps.a[0], bar, 0, k0);
@@ -101,13 +163,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (K == Kind::mxf4)
       tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);
   };
-  const int count = k_end - k_begin, ahead = min(count, q.stages);
   if (tid == 0) {
     for (int s = 0; s < q.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(a_ready, 8); // the quantising warps
     *abort_flag = 0;
     fence_mbarrier_init();
     // The producer's own barriers are ready: the first weights need not wait for the rest.
@@ -124,9 +186,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      for (int i = 0; i < ahead; ++i)
-        load_a(k_begin + i, i);
+      if (!direct) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (int i = 0; i < ahead; ++i)
+          load_a(k_begin + i, i);
+      }
       int issued = ahead, s = 0;
       uint32_t phase = 0;
       for (; issued < count; ++issued) {
@@ -136,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         load_b(k_begin + issued, s);
-        load_a(k_begin + issued, s);
+        if (!direct)
+          load_a(k_begin + issued, s);
         if (++s == q.stages) {
           s = 0;
           phase ^= 1;
@@ -155,6 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int s = 0;
       uint32_t phase = 0;
+      if (direct && !mbar_wait_bounded(a_ready, 0, p.timeout_ns)) {
+        atomicOr(&feed_error, 1u);
+        *abort_flag = 1;
+      }
       for (int kt = k_begin; kt < k_end; ++kt) {
         if (*abort_flag || !mbar_wait_bounded(&full[s], phase, p.timeout_ns)) {
           atomicOr(&feed_error, 1u);
@@ -162,12 +231,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         tc::fence_after();
-        const uint32_t a = sbase + s * stage_bytes, b = a + b_off;
+        const uint32_t base = ring + s * stage_bytes;
+        const int i = kt - k_begin;
+        const uint32_t a = direct ? sbase + i * q.a_bytes : base;
         if constexpr (K == Kind::f16)
-          stage_f16<1>(p, tmem, a, b, kt == k_begin);
+          stage_f16<1>(p, tmem, a, base + b_off, i == 0);
         else
-          stage_mxf4<1>(p, tmem, a, b, a + scale_off, tmem + kScaleCol + (s % 10) * kScaleCols,
-                        kt == k_begin);
+          stage_mxf4<1>(p, tmem, a, base + b_off,
+                        direct ? sbase + count * q.a_bytes + i * kScaleTile : base + scale_off,
+                        base + scale_b_off, tmem + kScaleCol + s * kScaleCols, i == 0);
         tc::mma_commit<1>(smem_u32(&empty[s]));
         if (++s == q.stages) {
           s = 0;
@@ -179,6 +251,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------- accumulator to shared memory
+    if constexpr (K == Kind::mxf4) {
+      if (direct) {
+        const int first = 8 * k_begin, last = 8 * k_end, thread = tid - 64;
+        unsigned char* scales = smem + count * q.a_bytes;
+        if (q.in.type == 0)
+          quantize_rows<__half>(q.in, p.m, first, last, smem, q.a_bytes, scales, thread, 256);
+        else if (q.in.type == 1)
+          quantize_rows<__nv_bfloat16>(q.in, p.m, first, last, smem, q.a_bytes, scales, thread,
+                                       256);
+        else
+          quantize_rows<float>(q.in, p.m, first, last, smem, q.a_bytes, scales, thread, 256);
+        // The tensor core reads shared memory through the async proxy.
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+          mbar_arrive(a_ready);
+      }
+    }
     const int quad = warp & 3, half = (warp - 2) >> 2;
     const bool ok = mbar_wait_bounded(acc_full, 0, p.timeout_ns * 4);
     if (!ok) {
@@ -310,7 +400,8 @@ long long cluster_capacity(F* kernel, int size, long long sms) {
 
 // `after`: launched behind a kernel of the same stream that allows programmatic overlap.
 template <Kind K, Epilogue E, class T>
-cudaError_t launch_split(const Maps& maps, const Params& p, bool after, cudaStream_t stream) {
+cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& in, bool after,
+                         cudaStream_t stream) {
   constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
   static std::atomic<uint64_t> done{0};
   const auto kernel = feed_split_kernel<K, E, T>;
@@ -318,29 +409,40 @@ cudaError_t launch_split(const Maps& maps, const Params& p, bool after, cudaStre
     return e;
   SplitParams q;
   q.p = p;
+  q.in = in;
+  const bool direct = in.x != nullptr;
   q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
-  const int stage = q.a_bytes + 2 * kPart + (K == Kind::mxf4 ? kScaleBytes : 0);
-  q.stages = std::min(K == Kind::mxf4 ? 10 : kSplitMaxStages, kSplitRing / stage);
   // Estimated time of a split, in us: a stage takes 0.75 when all SMs read from HBM and at least
   // 0.45 (one SM's rate); a wave of CTAs 2.5 to start, joining 1.  Clusters fit an SM count that
   // the hardware's grouping of SMs limits.
   const long long tiles = (p.n + kTileN - 1) / kTileN, sms = tc::sm_count();
   double best = 0;
-  q.splits = 1;
+  q.splits = 0;
   for (int s = 1; s <= 8 && s <= p.k_tiles; s *= 2) {
     const long long ctas = tiles * s, cap = s == 1 ? sms : cluster_capacity(kernel, s, sms);
     if (cap < s)
-      break;
+      continue;
     const double stage_us =
         std::max(0.45, 0.75 * static_cast<double>(std::min(ctas, cap)) / static_cast<double>(sms));
     const double t = static_cast<double>((ctas + cap - 1) / cap) *
                          (2.5 + stage_us * ((p.k_tiles + s - 1) / s)) +
                      (s > 1 ? 1.0 : 0.0);
-    if (s == 1 || t < best) {
+    // A quantised A has to fit, whatever the time.
+    const bool fits = !direct || ((p.k_tiles + s - 1) / s) *
+                                         (q.a_bytes + static_cast<int>(kScaleTile)) <=
+                                     kDirectBytes;
+    if (fits && (q.splits == 0 || t < best)) {
       best = t;
       q.splits = s;
     }
   }
+  if (q.splits == 0)
+    return cudaErrorInvalidValue;
+  const int most = (p.k_tiles + q.splits - 1) / q.splits; // stages of a CTA
+  q.ring = direct ? most * (q.a_bytes + static_cast<int>(kScaleTile)) : 0;
+  const int stage = (direct ? 0 : q.a_bytes) + 2 * kPart +
+                    (K == Kind::mxf4 ? (direct ? 2 : 3) * kScaleTile : 0);
+  q.stages = std::min(K == Kind::mxf4 ? 10 : kSplitMaxStages, (kSplitRing - q.ring) / stage);
   const long long grid = tiles * q.splits;
   if (grid > 0x7fffffffll)
     return cudaErrorInvalidConfiguration;

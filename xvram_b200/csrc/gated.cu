@@ -271,7 +271,7 @@ cudaError_t forward_16(const GatedProblem& q, void* out, long long ldo, cudaStre
   p.lds = q.ld_pre;
   if (split) {
     p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 128, 256);
-    return launch_split<Kind::f16, Epilogue::gated, T>(maps, p, false, stream);
+    return launch_split<Kind::f16, Epilogue::gated, T>(maps, p, DirectInput{}, false, stream);
   }
   return launch_16<Epilogue::gated, T>(maps, p, stream);
 }

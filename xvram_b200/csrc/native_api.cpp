@@ -168,7 +168,9 @@ xvram_status run_mxfp4(const xvram_b200_mxfp4_product_v1& d, bool gated) {
     return XVRAM_STATUS_INVALID_ARGUMENT;
   if (d.m == 0 || d.n == 0)
     return XVRAM_STATUS_SUCCESS;
-  if (!mxfp4_operand(d.x_codes, d.x_scales) || !d.out || d.ld_out < d.n ||
+  const bool direct = d.x && d.m <= XVRAM_B200_MXFP4_DIRECT_ROWS &&
+                      d.m * d.k <= XVRAM_B200_MXFP4_DIRECT_VALUES;
+  if ((!direct && !mxfp4_operand(d.x_codes, d.x_scales)) || !d.out || d.ld_out < d.n ||
       !element_aligned(d.out, d.out_type) ||
       (d.x && (d.ldx < d.k || !element_aligned(d.x, d.x_type))))
     return XVRAM_STATUS_INVALID_ARGUMENT;

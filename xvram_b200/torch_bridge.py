@@ -202,6 +202,7 @@ def _pack(padded: list, like: torch.Tensor, per: int, kind: int, index: int):
 
 
 _GATED_SIZE = ctypes.sizeof(Gated)
+_DIRECT_ROWS, _DIRECT_VALUES = 16, 65536  # XVRAM_B200_MXFP4_DIRECT_*: quantised inside the product
 _PRODUCT_SIZE = ctypes.sizeof(Mxfp4Product)
 
 
@@ -481,7 +482,8 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
             src, ldx, codes, scales, like = 0, 0, x.codes.data_ptr(), x.scales.data_ptr(), x.codes
         else:
             like, ldx = _rows(x)
-            src = like.data_ptr()
+            src, codes, scales = like.data_ptr(), 0, 0
+        if not quantised and (m > _DIRECT_ROWS or m * k > _DIRECT_VALUES):
             size = m * ((k + 31) // 32) * 16
             buffer = like.new_empty((size + (m + 127) // 128 * ((k + 127) // 128) * 512,),
                                     dtype=torch.uint8)
