@@ -7,20 +7,17 @@
 //   16-bit, HALVES = 1  a tile is 256 rows; two accumulators fill TMEM and alternate, so the
 //               epilogue of a tile runs under the next tile's MMAs;
 //   16-bit, HALVES = 2  a tile is 512 rows, 256 per CTA, both accumulators over the same B: a
-//               quarter less operand traffic per FLOP.  The epilogue first empties an
-//               accumulator into registers and hands it back, and the next tile's first stages
-//               run on accumulator 0 alone (kAhead stages) before accumulator 1 is needed, so
-//               the MMAs wait only for the first emptying;
+//               quarter less operand traffic per FLOP.  The MMAs wait for the epilogues, which
+//               run side by side; the next tile's first stages run on accumulator 0 alone
+//               (kAhead stages) before accumulator 1 is needed;
 //   MXFP4       a tile is 256 rows with one accumulator, emptied into registers first; the
 //               other TMEM columns hold the stages' scales (each CTA's own A rows, all B rows).
 //
 //   warp 0      one lane per CTA: TMA loads into the stage ring, completion on the leader's
 //               barrier;
 //   warp 1      leader: one lane issues the MMAs and commits stages and accumulators to both CTAs;
-//   warps 2..9  epilogue per CTA, two warps per TMEM lane quarter splitting the columns; their
-//               arrivals on the leader's barrier hand the accumulator back.  Results go
-//               through a 32-row x 128-byte block of shared memory per warp, so that global
-//               stores are whole 128-byte lines.
+//   warps 2..   epilogue per CTA, 8 warps per accumulator: two per TMEM lane quarter, splitting
+//               the columns; their arrivals on the leader's barrier hand the accumulator back.
 #pragma once
 
 #include "feed_common.cuh"
@@ -34,6 +31,9 @@ struct PairShape {
   static constexpr int kSlots = K == Kind::mxf4 ? 1 : 2; // accumulators
   static constexpr uint32_t kScales = (HALVES + 1) * kPart; // offset of a stage's scales
   static constexpr uint32_t kStage = kScales + (K == Kind::mxf4 ? kScaleBytes : 0);
+  // 16-bit: two groups of 8 epilogue warps, a group per accumulator; MXFP4: one.
+  static constexpr int kGroups = kSlots;
+  static constexpr int kThreads = 64 + 256 * kGroups;
   static constexpr int kSmem = kStages * kStage + 8 * kStageBlock + 1024 + 256;
 };
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ void tile_origin(const Params& p, int t, int rows, in
 }
 
 template <Kind K, Epilogue E, class T, int HALVES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<K, HALVES>::kThreads, 1)
     feed_pair_kernel(const __grid_constant__ Maps maps, const Params p) {
   constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
   using Shape = PairShape<K, HALVES>;
@@ -245,9 +245,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- epilogue
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    const uint32_t release = tc::cluster_addr(smem_u32(acc_empty), 0);
-    unsigned char* block = blocks + (warp - 2) * kStageBlock;
+    // Group g of 8 warps takes accumulator g's units; a unit is a tile's (half's) accumulator.
+    const int quad = warp & 3, half = ((warp - 2) >> 2) & 1, group = (warp - 2) >> 3;
+    const uint32_t release = tc::cluster_addr(smem_u32(acc_empty), 0) + 8 * group;
     int unit = 0;
     bool stop = false;
     for (int t = first; t < tiles && !stop; t += pairs) {
@@ -255,9 +255,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tile_origin(p, t, 256 * HALVES, kTileN, batch, m0, n0);
       T* out = static_cast<T*>(p.out[batch]);
       for (int i = 0; i < HALVES; ++i, ++unit) {
-        const int buf = unit % kSlots;
+        if (unit % Shape::kGroups != group)
+          continue;
         const int row0 = m0 + 128 * (HALVES * static_cast<int>(rank) + i) + 32 * quad;
-        const bool ok = mbar_wait_bounded(&acc_full[buf], (unit / kSlots) & 1,
+        const bool ok = mbar_wait_bounded(&acc_full[group], (unit / kSlots) & 1,
                                           p.timeout_ns * 4);
         if (!ok) {
           atomicOr(&feed_error, 8u);
@@ -268,14 +269,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           stop = true;
           break;
         }
-        const uint32_t t_row = tmem + 256 * buf + (static_cast<uint32_t>(32 * quad) << 16);
-        float r[128];
-        load_accumulator<E>(t_row, half, r);
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0)
-          tc::mbar_arrive_cluster(release + 8 * buf);
-        finish_rows<E, T>(p, r, row0, n0 + half * (kTileN / 2), out, block);
+        const uint32_t t_row = tmem + 256 * group + (static_cast<uint32_t>(32 * quad) << 16);
+        const auto hand_back = [&] {
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0)
+            tc::mbar_arrive_cluster(release);
+        };
+        const int col = n0 + half * (kTileN / 2);
+        if constexpr (K == Kind::mxf4) {
+          // One accumulator: emptied into registers, so that the next tile's MMAs wait only for that.
+          float r[128];
+          load_accumulator<E>(t_row, half, r);
+          hand_back();
+          finish_rows<E, T>(p, r, row0, col, out, blocks + (warp - 2) * kStageBlock);
+        } else {
+          finish_unit<E, T>(p, t_row, half, row0, col, out, blocks + (warp - 2) * kSubBlock,
+                            hand_back);
+        }
       }
     }
   }
@@ -304,7 +315,7 @@ cudaError_t launch_pairs(const Maps& maps, Params p, cudaStream_t stream) {
   if (tiles <= 0 || tiles > 0x7fffffffll)
     return cudaErrorInvalidConfiguration;
   const int pairs = static_cast<int>(std::min<long long>(tiles, tc::sm_count() / 2));
-  kernel<<<2 * pairs, kThreads, smem, stream>>>(maps, p);
+  kernel<<<2 * pairs, PairShape<K, HALVES>::kThreads, smem, stream>>>(maps, p);
   return cudaGetLastError();
 }
 
