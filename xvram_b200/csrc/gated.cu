@@ -236,15 +236,15 @@ Params base_params(bool bf16, int m, int n, int k_tiles, bool a_mn, bool b_mn, i
   return p;
 }
 
-// The pair kernel, with 512-row tiles where their waves cost less: one runs in 1.85 times a
-// 256-row tile's time (8192 x 4096 x 8192, seconds of it back to back under the power cap: 832 us
-// against 859; 2048 rows, 4 waves against 7: 231 against 222).
+// The pair kernel, with 512-row tiles where their waves cost less: one runs in 1.75 times a
+// 256-row tile's time (8192 x 4096 x 8192, seconds of it back to back under the power cap: 824 us
+// against 868; 2048 rows, 4 waves against 7: 225 against 222).
 template <Epilogue E, class T>
 cudaError_t launch_16(const Maps& maps, const Params& p, cudaStream_t stream) {
   const long long pairs = tc::sm_count() / 2, cols = static_cast<long long>(p.batches) * p.tiles_n;
   const long long one = (cols * ((p.m + 255) / 256) + pairs - 1) / pairs;
   const long long two = (cols * ((p.m + 511) / 512) + pairs - 1) / pairs;
-  return 1.85 * two < one ? launch_pairs<Kind::f16, E, T, 2>(maps, p, stream)
+  return 1.75 * two < one ? launch_pairs<Kind::f16, E, T, 2>(maps, p, stream)
                           : launch_pairs<Kind::f16, E, T, 1>(maps, p, stream);
 }
 
