@@ -404,7 +404,7 @@ typedef struct xvram_b200_gated_v1 {
   uint32_t activation;  /* XVRAM_B200_GATE_* */
   uint32_t x_transposed, w_transposed;
   uint32_t reserved0;
-  int64_t m, h, k; /* m and h >= 0, k >= 1 */
+  int64_t m, h, k; /* m and h >= 0, k >= 1; at most INT32_MAX - 511 */
   uint64_t x, w_gate, w_up;
   int64_t ldx, ld_gate, ld_up;
   uint64_t bias_gate, bias_up;
@@ -487,7 +487,7 @@ typedef struct xvram_b200_mxfp4_product_v1 {
   uint32_t struct_size; /* sizeof(xvram_b200_mxfp4_product_v1) */
   uint32_t x_type, out_type; /* XVRAM_DATA_FP16, _BF16 or _FP32 */
   uint32_t activation; /* linear: XVRAM_B200_ACTIVATION_*; gated: XVRAM_B200_GATE_* */
-  int64_t m, n, k; /* m and n >= 0, k >= 1 */
+  int64_t m, n, k; /* m and n >= 0, k >= 1; at most INT32_MAX - 511 */
   uint64_t x;
   int64_t ldx;
   uint64_t x_codes, x_scales;

@@ -76,7 +76,8 @@ def gated(**changes):
 
 @pytest.mark.parametrize("changes", [
     {"struct_size": 8}, {"data_type": 3}, {"activation": 5}, {"x_transposed": 2},
-    {"w_transposed": 7}, {"m": -1}, {"h": -1}, {"k": 0}, {"m": 1 << 31}, {"x": 0}, {"w_gate": 0},
+    {"w_transposed": 7}, {"m": -1}, {"h": -1}, {"k": 0}, {"m": 1 << 31}, {"h": (1 << 31) - 511},
+    {"x": 0}, {"w_gate": 0},
     {"w_up": 0}, {"ldx": 15}, {"ld_gate": 15}, {"ld_up": 3}, {"x": 4097}, {"bias_gate": 3},
     {"pre_gate": 4096}, {"pre_gate": 4096, "pre_up": 4104, "ld_pre": 8},
     {"pre_gate": 4096, "pre_up": 8192, "ld_pre": 10},

@@ -114,12 +114,15 @@ bool element_aligned(uint64_t p, uint32_t data_type) {
   return p % (data_type == XVRAM_DATA_FP32 ? 4 : 2) == 0;
 }
 
+// Sizes round up to whole tiles (512 at most) as ints.
+constexpr int64_t kMostRows = INT32_MAX - 511;
+
 // The checked problem; false when an argument is invalid.  `operands` also checks the pointers
 // and leading dimensions (the workspace query has none).
 bool gated_problem(const xvram_b200_gated_v1& d, bool operands, GatedProblem* q) {
   if (d.struct_size < sizeof(d) || d.data_type > XVRAM_DATA_FP32 ||
       d.activation > XVRAM_B200_GATE_SIGMOID || d.x_transposed > 1 || d.w_transposed > 1 ||
-      d.m < 0 || d.h < 0 || d.k < 1 || d.m > INT32_MAX || d.h > INT32_MAX || d.k > INT32_MAX)
+      d.m < 0 || d.h < 0 || d.k < 1 || d.m > kMostRows || d.h > kMostRows || d.k > kMostRows)
     return false;
   if (operands && d.m > 0 && d.h > 0) {
     const int64_t wx = d.x_transposed ? d.m : d.k, ww = d.w_transposed ? d.h : d.k;
@@ -153,9 +156,8 @@ bool gated_problem(const xvram_b200_gated_v1& d, bool operands, GatedProblem* q)
   return true;
 }
 
-// Columns are at most 2^31 - 32, so that a padded row's length is an int.
 bool mxfp4_size(int64_t rows, int64_t cols) {
-  return rows >= 0 && cols >= 0 && rows <= INT32_MAX - 127 && cols <= INT32_MAX - 255;
+  return rows >= 0 && cols >= 0 && rows <= kMostRows && cols <= kMostRows;
 }
 bool mxfp4_operand(uint64_t codes, uint64_t scales) {
   return codes && scales && codes % 16 == 0 && scales % 16 == 0;
