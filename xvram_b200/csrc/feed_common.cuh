@@ -584,7 +584,7 @@ __device__ __forceinline__ void add_bias_rows(unsigned char* block, const void* 
 }
 
 // The loaded accumulator half to results: 64 gated or 128 plain columns from `col` on of the
-// warp's rows row0...
+// warp's rows row0.. (the MXFP4 products', which keep no pre-activations).
 template <Epilogue E, class T>
 __device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], int row0, int col,
                                             T* out, unsigned char* block) {
@@ -600,13 +600,6 @@ __device__ __forceinline__ void finish_rows(const Params& p, float (&v)[128], in
     }
     add_bias_rows<T, 64>(block, p.bias0, col, p.n, g);
     add_bias_rows<T, 64>(block, p.bias1, col, p.n, u);
-    if (p.save_gate) {
-#pragma unroll
-      for (int i = 0; i < 64; i += 32) {
-        store_block(block, g, i, p.save_gate, p.lds, row0, col + i, p.m, p.n, 16);
-        store_block(block, u, i, p.save_up, p.lds, row0, col + i, p.m, p.n, 16);
-      }
-    }
     gate<sizeof(T) == 2>(p.act, g, u);
 #pragma unroll
     for (int i = 0; i < 64; i += kBlockCols)

@@ -240,13 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage_mxf4<1>(p, tmem, a, base + b_off,
                         direct ? sbase + count * q.a_bytes + i * kScaleTile : base + scale_off,
                         base + scale_b_off, tmem + kScaleCol + s * kScaleCols, i == 0);
-        tc::mma_commit<1>(smem_u32(&empty[s]));
+        tc::mma_commit(smem_u32(&empty[s]));
         if (++s == q.stages) {
           s = 0;
           phase ^= 1;
         }
       }
-      tc::mma_commit<1>(smem_u32(acc_full));
+      tc::mma_commit(smem_u32(acc_full));
     }
     __syncwarp();
   } else {

@@ -66,16 +66,10 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
 
 // Arrives on the mbarrier at shared::cluster address `bar` once every tensor-core operation
 // issued so far by this thread has completed.
-template <int PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  if constexpr (PAIR == 2)
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-        : "memory");
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
 }
 
 // mma_commit of a pair's leader to the barriers at this shared::cta offset in both CTAs.

@@ -324,8 +324,8 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     if dh.shape != (m, h) or dh.dtype != dtype or dh.device != device:
         raise ValueError(f"dh must be a ({m}, {h}) {dtype} tensor on {device}")
     index, size = device.index, 4 if kind == sdk.FP32 else 2
-    with torch.no_grad(), _on_device(index):
-        dh, lddh = _rows(dh)
+    with _on_device(index):
+        dh, lddh = _rows(dh.detach() if dh.requires_grad else dh)
         dx = dh.new_empty((m, k)) if needs[0] else None
         dwg = dh.new_empty((h, k)) if needs[1] else None
         dwu = dh.new_empty((h, k)) if needs[2] else None
@@ -351,8 +351,9 @@ class _GatedLinear(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("gated_linear has no second derivative")
         saved = GatedSaved(ctx.saved_tensors, ctx.layout)
         return (*gated_linear_backward(dh, saved, ctx.needs_input_grad), None)
 
