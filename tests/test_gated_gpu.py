@@ -107,3 +107,11 @@ def test_every_operand_layout(kind, shape):
     check_gradients((x, wg, layouts(wu)[1], bg, bu), "silu", dh)  # stored in different ways
     for dhv in layouts(dh)[1:] + [dh[:1].expand(m, h)]:
         check_gradients((x, wg, wu, bg, bu), "silu", dhv)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 6, 7, 8, 9, 17])
+@pytest.mark.parametrize("kind", TYPES)
+def test_each_number_of_few_rows(kind, m):
+    """One or two features per warp, rows of whole 16 bytes, with a rest, and unaligned."""
+    for h, k in ((40, 512), (40, 516), (2400, 515), (2401, 264)):
+        check_forward(problem(kind, m, h, k, 60 + m), "silu")

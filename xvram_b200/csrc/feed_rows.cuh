@@ -51,9 +51,10 @@ __device__ __forceinline__ void load_stream(const T* p, Values<T, N>& d) {
 // VEC: values a lane reads at once (16 bytes' worth, or 1 when rows are not 16-byte aligned).
 template <class T, int MR, int HPW, int VEC>
 __global__ void __launch_bounds__(256, 2) feed_rows_kernel(const RowsParams p) {
-  constexpr int NV = 2 * HPW * MR;
-  static_assert((NV & (NV - 1)) == 0 && NV <= 32, "sums are a power of two");
-  constexpr int UNROLL = 4;
+  constexpr int kSums = 2 * HPW * MR; // and zeros up to a power of two, for the butterfly
+  constexpr int NV = kSums <= 2 ? 2 : kSums <= 4 ? 4 : kSums <= 8 ? 8 : kSums <= 16 ? 16 : 32;
+  static_assert(kSums <= NV, "at most 32 sums");
+  constexpr int UNROLL = VEC > 1 ? 4 : NV > 2 ? 8 : 6;
   __shared__ float sums[8][NV];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long h0 = (blockIdx.x * 8ll + warp) * HPW;
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(256, 2) feed_rows_kernel(const RowsParams p) {
 // 4096 x 8192 2 rows 26.2 and 30.8, where x costs less.
 template <class T, int VEC>
 cudaError_t launch_rows(const RowsParams& p, cudaStream_t stream) {
-  const int mr = p.m >= 5 ? 8 : p.m >= 3 ? 4 : p.m;
+  const int mr = p.m >= 7 ? 8 : p.m;
   const bool two = mr >= (sizeof(T) == 4 ? 2 : 3) && p.h >= 2 * 8 * tc::sm_count();
   const unsigned per = two ? 16 : 8;
   const dim3 grid((p.h + per - 1) / per, (p.m + mr - 1) / mr);
@@ -199,11 +200,17 @@ cudaError_t launch_rows(const RowsParams& p, cudaStream_t stream) {
   switch (mr) {
   case 1: return run(feed_rows_kernel<T, 1, 1, VEC>);
   case 2: return two ? run(feed_rows_kernel<T, 2, 2, VEC>) : run(feed_rows_kernel<T, 2, 1, VEC>);
+  case 3: return two ? run(feed_rows_kernel<T, 3, 2, VEC>) : run(feed_rows_kernel<T, 3, 1, VEC>);
   case 4: return two ? run(feed_rows_kernel<T, 4, 2, VEC>) : run(feed_rows_kernel<T, 4, 1, VEC>);
   default:
     // 16-bit operands of more rows run on the tensor cores.
-    if constexpr (sizeof(T) == 4)
+    if constexpr (sizeof(T) == 4) {
+      if (mr == 5)
+        return two ? run(feed_rows_kernel<T, 5, 2, VEC>) : run(feed_rows_kernel<T, 5, 1, VEC>);
+      if (mr == 6)
+        return two ? run(feed_rows_kernel<T, 6, 2, VEC>) : run(feed_rows_kernel<T, 6, 1, VEC>);
       return two ? run(feed_rows_kernel<T, 8, 2, VEC>) : run(feed_rows_kernel<T, 8, 1, VEC>);
+    }
     return cudaErrorInvalidValue;
   }
 }
