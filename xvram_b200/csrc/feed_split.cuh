@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sbase = smem_u32(smem), ring = sbase + q.ring;
   const auto load_b = [&](int kt, int s) {
     const uint32_t bar = smem_u32(&full[s]), base = ring + s * stage_bytes;
-    const int k0 = kt * kElems;
+    const int seg = kt >= p.k_split, k0 = (kt - (seg ? p.k_split : 0)) * kElems;
     mbar_arrive_expect_tx(&full[s], stage_bytes);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : 0];
+      const CUtensorMap* mb = &maps.b[E == Epilogue::gated ? j : seg];
       const int row = E == Epilogue::gated ? n0 : n0 + 128 * j;
       const uint32_t d = base + b_off + j * kPart;
       if (K == Kind::f16 && p.b_mn) {
@@ -153,12 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const auto load_a = [&](int kt, int s) {
     const uint32_t bar = smem_u32(&full[s]), base = ring + s * stage_bytes;
-    const int k0 = kt * kElems;
+    const int seg = kt >= p.k_split, k0 = (kt - (seg ? p.k_split : 0)) * kElems;
     if (K == Kind::f16 && p.a_mn) {
-      tc::tma_load<1>(base, &maps.a[0], bar, 0, k0);
-      tc::tma_load<1>(base + kPart / 2, &maps.a[0], bar, 64, k0);
+      tc::tma_load<1>(base, &maps.a[seg], bar, 0, k0);
+      tc::tma_load<1>(base + kPart / 2, &maps.a[seg], bar, 64, k0);
     } else {
-      tc::tma_load<1>(base, &maps.a[0], bar, k0, 0);
+      tc::tma_load<1>(base, &maps.a[seg], bar, k0, 0);
     }
     if constexpr (K == Kind::mxf4)
       tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);

@@ -295,9 +295,10 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
   if (d.dx) {
     // dx (m x k): A = dg, then du, along h; B = Wg, then Wu, whose rows are the inputs.
     Maps maps;
-    const bool b_mn = !q.w_transposed;
-    if (!operand_map(&maps.a[0], bf16, dg, q.m, q.h, ldd, false) ||
-        !operand_map(&maps.a[1], bf16, du, q.m, q.h, ldd, false) ||
+    const bool b_mn = !q.w_transposed, split = q.m <= 128;
+    const uint32_t box = split ? split_rows(q.m) : 128;
+    if (!operand_map(&maps.a[0], bf16, dg, q.m, q.h, ldd, false, box) ||
+        !operand_map(&maps.a[1], bf16, du, q.m, q.h, ldd, false, box) ||
         !operand_map(&maps.b[0], bf16, q.w_gate, q.k, q.h, q.ld_gate, b_mn) ||
         !operand_map(&maps.b[1], bf16, q.w_up, q.k, q.h, q.ld_up, b_mn))
       return cudaErrorInvalidValue;
@@ -307,8 +308,14 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[0] = p.out[1] = d.dx;
     p.ldo = d.lddx;
     p.unit = store_unit<T>(d.dx, d.lddx);
-    if (cudaError_t e = launch_16<Epilogue::plain, T>(maps, p, stream);
-        e != cudaSuccess)
+    cudaError_t e;
+    if (split) { // bound by reading the weights
+      p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 128, 256);
+      e = launch_split<Kind::f16, Epilogue::plain, T>(maps, p, DirectInput{}, false, stream);
+    } else {
+      e = launch_16<Epilogue::plain, T>(maps, p, stream);
+    }
+    if (e != cudaSuccess)
       return e;
   }
   if (d.dw_gate || d.dw_up) {
