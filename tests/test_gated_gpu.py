@@ -115,3 +115,11 @@ def test_each_number_of_few_rows(kind, m):
     """One or two features per warp, rows of whole 16 bytes, with a rest, and unaligned."""
     for h, k in ((40, 512), (40, 516), (2400, 515), (2401, 264)):
         check_forward(problem(kind, m, h, k, 60 + m), "silu")
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(140, 4000, 300), (300, 2100, 520), (1021, 2730, 77)])
+def test_gradients_with_few_tiles_and_a_long_sum(kind, shape):
+    """dx has few tiles and K = 2 out: it runs over several row tiles with K split."""
+    m, h, k = shape
+    check_gradients(problem(kind, m, h, k, 70), "sigmoid", fu.normal((m, h), kind, 71))

@@ -1,5 +1,5 @@
-// feed_split.cuh -- the tensor-core kernel of the feed-forward operators for at most 128 rows
-// (operands, epilogues and the accumulator's columns: feed_common.cuh).
+// feed_split.cuh -- the tensor-core kernel of the feed-forward operators for at most 128 rows, and
+// for more where CTA pairs would find too few tiles (operands, epilogues and the accumulator's columns: feed_common.cuh).
 //
 // Bound by reading the weights from HBM: a 128 x 256 accumulator takes all rows of A, so each
 // weight is read once, and M = 128 MMAs on fewer rows still finish inside the time of the
@@ -118,7 +118,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int rank = q.splits > 1 ? static_cast<int>(tc::cluster_rank()) : 0;
-  const int n0 = static_cast<int>(blockIdx.x / q.splits) * kTileN;
+  // Row tiles run fastest: those of one weight tile work at the same time.
+  const int tile = static_cast<int>(blockIdx.x / q.splits);
+  const int m0 = tile % p.tiles_m * 128, n0 = tile / p.tiles_m * kTileN;
+  const int rows = min(128, p.m - m0);
   const int k_begin = static_cast<int>(static_cast<long long>(p.k_tiles) * rank / q.splits);
   const int k_end = static_cast<int>(static_cast<long long>(p.k_tiles) * (rank + 1) / q.splits);
   const bool direct = K == Kind::mxf4 && q.in.x;
@@ -155,13 +158,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t bar = smem_u32(&full[s]), base = ring + s * stage_bytes;
     const int seg = kt >= p.k_split, k0 = (kt - (seg ? p.k_split : 0)) * kElems;
     if (K == Kind::f16 && p.a_mn) {
-      tc::tma_load<1>(base, &maps.a[seg], bar, 0, k0);
-      tc::tma_load<1>(base + kPart / 2, &maps.a[seg], bar, 64, k0);
+      tc::tma_load<1>(base, &maps.a[seg], bar, m0, k0);
+      tc::tma_load<1>(base + kPart / 2, &maps.a[seg], bar, m0 + 64, k0);
     } else {
-      tc::tma_load<1>(base, &maps.a[seg], bar, k0, 0);
+      tc::tma_load<1>(base, &maps.a[seg], bar, k0, m0);
     }
     if constexpr (K == Kind::mxf4)
-      tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, 0);
+      tc::tma_load<1>(base + scale_off, &maps.scale_a, bar, kt * 256, m0 / 128);
   };
   if (tid == 0) {
     for (int s = 0; s < q.stages; ++s) {
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       *abort_flag = 1;
     }
     tc::fence_after();
-    if (32 * quad < p.m && __all_sync(0xffffffffu, ok && !*abort_flag)) {
+    if (32 * quad < rows && __all_sync(0xffffffffu, ok && !*abort_flag)) {
       const int row = 32 * quad + lane;
       const uint32_t t_row = tmem + (static_cast<uint32_t>(32 * quad) << 16);
       float* dst = reinterpret_cast<float*>(smem) + row * kPitch;
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_ld16(t_row + 128 * half + c, r[0]);
         tc::tmem_ld16(t_row + 128 * half + c + 16, r[1]);
         tc::tmem_wait_ld();
-        if (row < p.m) {
+        if (row < rows) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<uint4*>(dst + 128 * half + c + i) =
@@ -310,8 +313,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // ---------------------------------------------------------- reduce and finish
   const int cols = kTileN / q.splits; // a multiple of 16
   const int groups = cols / 4;
-  T* out = static_cast<T*>(p.out[0]);
-  for (int i = tid; i < p.m * groups; i += kThreads) {
+  T* out = static_cast<T*>(p.out[0]) + m0 * p.ldo;
+  const long long kept = m0 * p.lds;
+  for (int i = tid; i < rows * groups; i += kThreads) {
     const int r = i / groups, c = rank * cols + (i - r * groups) * 4;
     const int col = n0 + c;
     if (col >= p.n)
@@ -334,8 +338,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (col + j < p.n) {
-            p.save_gate[r * p.lds + col + j] = v[j];
-            p.save_up[r * p.lds + col + j] = w[j];
+            p.save_gate[kept + r * p.lds + col + j] = v[j];
+            p.save_up[kept + r * p.lds + col + j] = w[j];
           }
       }
       gate<sizeof(T) == 2>(p.act, v, w);
@@ -398,26 +402,30 @@ long long cluster_capacity(F* kernel, int size, long long sms) {
   return static_cast<long long>(clusters - 1) * size;
 }
 
-// `after`: launched behind a kernel of the same stream that allows programmatic overlap.
 template <Kind K, Epilogue E, class T>
-cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& in, bool after,
-                         cudaStream_t stream) {
-  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
+cudaError_t allow_split() {
   static std::atomic<uint64_t> done{0};
+  return tc::allow_smem(feed_split_kernel<K, E, T>, kSplitSmem, done);
+}
+
+// The cluster size with the least estimated time, and that time in us: a stage takes 0.75 when all SMs
+// read from HBM and at least 0.45 (one SM's rate); a wave of CTAs 2.5 to start, joining 1.  Clusters
+// fit an SM count that the hardware's grouping of SMs limits.  A quantised A (a_bytes per stage)
+// has to fit, whatever the time; 0 splits if it does not.
+struct Split {
+  int splits;
+  double us;
+};
+template <Kind K, Epilogue E, class T>
+Split choose_split(const Params& p, int a_bytes) {
+  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
   const auto kernel = feed_split_kernel<K, E, T>;
-  if (cudaError_t e = tc::allow_smem(kernel, kSplitSmem, done); e != cudaSuccess)
-    return e;
-  SplitParams q;
-  q.p = p;
-  q.in = in;
-  const bool direct = in.x != nullptr;
-  q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
-  // Estimated time of a split, in us: a stage takes 0.75 when all SMs read from HBM and at least
-  // 0.45 (one SM's rate); a wave of CTAs 2.5 to start, joining 1.  Clusters fit an SM count that
-  // the hardware's grouping of SMs limits.
-  const long long tiles = (p.n + kTileN - 1) / kTileN, sms = tc::sm_count();
-  double best = 0;
-  q.splits = 0;
+  const long long tiles =
+      static_cast<long long>((p.m + 127) / 128) * ((p.n + kTileN - 1) / kTileN);
+  const long long sms = tc::sm_count();
+  Split best{0, 0};
+  if (allow_split<K, E, T>() != cudaSuccess) // the capacity query needs it too
+    return best;
   for (int s = 1; s <= 8 && s <= p.k_tiles; s *= 2) {
     const long long ctas = tiles * s, cap = s == 1 ? sms : cluster_capacity(kernel, s, sms);
     if (cap < s)
@@ -427,15 +435,30 @@ cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& i
     const double t = static_cast<double>((ctas + cap - 1) / cap) *
                          (2.5 + stage_us * ((p.k_tiles + s - 1) / s)) +
                      (s > 1 ? 1.0 : 0.0);
-    // A quantised A has to fit, whatever the time.
-    const bool fits = !direct || ((p.k_tiles + s - 1) / s) *
-                                         (q.a_bytes + static_cast<int>(kScaleTile)) <=
-                                     kDirectBytes;
-    if (fits && (q.splits == 0 || t < best)) {
-      best = t;
-      q.splits = s;
-    }
+    const bool fits = !a_bytes || ((p.k_tiles + s - 1) / s) *
+                                          (a_bytes + static_cast<int>(kScaleTile)) <=
+                                      kDirectBytes;
+    if (fits && (best.splits == 0 || t < best.us))
+      best = {s, t};
   }
+  return best;
+}
+
+// `after`: launched behind a kernel of the same stream that allows programmatic overlap.
+template <Kind K, Epilogue E, class T>
+cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& in, bool after,
+                         cudaStream_t stream) {
+  constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
+  const auto kernel = feed_split_kernel<K, E, T>;
+  if (cudaError_t e = allow_split<K, E, T>(); e != cudaSuccess)
+    return e;
+  SplitParams q;
+  q.p = p;
+  q.in = in;
+  const bool direct = in.x != nullptr;
+  q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
+  q.p.tiles_m = (p.m + 127) / 128;
+  q.splits = choose_split<K, E, T>(p, direct ? q.a_bytes : 0).splits;
   if (q.splits == 0)
     return cudaErrorInvalidValue;
   const int most = (p.k_tiles + q.splits - 1) / q.splits; // stages of a CTA
@@ -443,7 +466,8 @@ cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& i
   const int stage = (direct ? 0 : q.a_bytes) + 2 * kPart +
                     (K == Kind::mxf4 ? (direct ? 2 : 3) * kScaleTile : 0);
   q.stages = std::min(K == Kind::mxf4 ? 10 : kSplitMaxStages, (kSplitRing - q.ring) / stage);
-  const long long grid = tiles * q.splits;
+  const long long grid =
+      static_cast<long long>(q.p.tiles_m) * ((p.n + kTileN - 1) / kTileN) * q.splits;
   if (grid > 0x7fffffffll)
     return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t config{};

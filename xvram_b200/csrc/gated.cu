@@ -295,8 +295,8 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
   if (d.dx) {
     // dx (m x k): A = dg, then du, along h; B = Wg, then Wu, whose rows are the inputs.
     Maps maps;
-    const bool b_mn = !q.w_transposed, split = q.m <= 128;
-    const uint32_t box = split ? split_rows(q.m) : 128;
+    const bool b_mn = !q.w_transposed;
+    const uint32_t box = split_rows(q.m);
     if (!operand_map(&maps.a[0], bf16, dg, q.m, q.h, ldd, false, box) ||
         !operand_map(&maps.a[1], bf16, du, q.m, q.h, ldd, false, box) ||
         !operand_map(&maps.b[0], bf16, q.w_gate, q.k, q.h, q.ld_gate, b_mn) ||
@@ -308,8 +308,14 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     p.out[0] = p.out[1] = d.dx;
     p.ldo = d.lddx;
     p.unit = store_unit<T>(d.dx, d.lddx);
+    // K is 2 h, so few tiles take long: split it up to 128 rows, and above where that is
+    // estimated to beat the pairs' waves at 0.3 us a stage.
+    const long long pairs = tc::sm_count() / 2;
+    const long long waves =
+        (static_cast<long long>(p.tiles_n) * ((q.m + 255) / 256) + pairs - 1) / pairs;
     cudaError_t e;
-    if (split) { // bound by reading the weights
+    if (q.m <= 128 || choose_split<Kind::f16, Epilogue::plain, T>(p, 0).us <
+                          static_cast<double>(waves) * (3.0 + 0.3 * p.k_tiles)) {
       p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 128, 256);
       e = launch_split<Kind::f16, Epilogue::plain, T>(maps, p, DirectInput{}, false, stream);
     } else {
