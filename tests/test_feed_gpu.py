@@ -264,3 +264,57 @@ def test_a_run_of_layers(kind):
     fu.within(yq, ref, fu.acc(h) * (hv.abs() @ v[2].abs().t()) + fu.HALF[kind] * ref.abs() +
               fu.TINY[kind], "4-bit down")
     assert xd.kernel_status() == 0
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_only_the_wanted_gradients(kind):
+    """Each subset of the gradients has the bits that all of them together have."""
+    x, (wg, wu) = fu.normal((150, 88), kind, 1), weights(kind, 104, 88, 2)
+    b = fu.normal((104,), kind, 4)
+    dh = fu.normal((150, 104), kind, 5)
+    _, saved = tb.gated_linear_forward(x, wg, wu, b, b, "gelu_tanh")
+    want = tb.gated_linear_backward(dh, saved)
+    for bits in range(32):
+        needs = tuple(bool(bits >> i & 1) for i in range(5))
+        got = tb.gated_linear_backward(dh, saved, needs)
+        for n, g, w in zip(needs, got, want):
+            assert (g is None) if not n else torch.equal(g, w)
+    frozen = wg.clone().requires_grad_()  # autograd asks for one weight's gradient alone
+    tb.gated_linear(x, frozen, wu, b, b, "gelu_tanh").backward(dh)
+    assert torch.equal(frozen.grad, want[1])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_empty_batches_of_odd_sizes(kind):
+    x = torch.empty((0, 9), dtype=kind, device="cuda", requires_grad=True)
+    wg, wu = (w.requires_grad_() for w in weights(kind, 7, 9, 1))
+    tb.gated_linear(x, wg, wu).sum().backward()
+    assert x.grad.shape == (0, 9) and not bool(wg.grad.any()) and not bool(wu.grad.any())
+    q = tb.quantize_mxfp4(wg.detach())
+    assert tb.gated_linear_mxfp4(x.detach(), q, q).shape == (0, 7)
+
+
+def test_two_threads_at_once():
+    """Calls from two host threads on streams of their own give what they give alone."""
+    import threading
+    kind = torch.bfloat16
+    x, (wg, wu) = fu.normal((60, 136), kind, 1), weights(kind, 264, 136, 2)
+    q = [tb.quantize_mxfp4(w) for w in (wg, wu)]
+    want = (tb.gated_linear(x, wg, wu), tb.gated_linear_mxfp4(x, *q), tb.linear_mxfp4(x[:3], q[0]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                got = (tb.gated_linear(x, wg, wu), tb.gated_linear_mxfp4(x, *q),
+                       tb.linear_mxfp4(x[:3], q[0]))
+                s.synchronize()
+                wrong.extend(i for i, (a, b) in enumerate(zip(got, want)) if not torch.equal(a, b))
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and xd.kernel_status() == 0
