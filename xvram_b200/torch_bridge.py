@@ -229,13 +229,49 @@ def _check_gated(x, w_gate, w_up, dtype: torch.dtype, device: torch.device) -> N
 
 
 class GatedSaved:
-    """What `gated_linear_backward` needs of a forward pass: the operands as the kernels read
-    them (x, w_gate, w_up, or the buffer that holds their padded copies) and the FP32
-    pre-activations (2, batch, out), with their layout."""
-    __slots__ = ("tensors", "layout")
+    """What `gated_linear_backward` needs of a forward pass: x, w_gate and w_up (or copies that
+    the kernels read without another one) and the FP32 pre-activations (2, batch, out padded to
+    whole 16 bytes), and the problem: (element type, activation, batch, out, in, torch type,
+    device)."""
+    __slots__ = ("tensors", "problem")
 
-    def __init__(self, tensors, layout):
-        self.tensors, self.layout = tensors, layout
+    def __init__(self, tensors, problem):
+        self.tensors, self.problem = tensors, problem
+
+
+def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int):
+    """x and the weights as the kernels read them: three (buffer, element offset, leading
+    dimension, padded) and whether x and the weights are transposed.  Not padded: the buffer is
+    the tensor itself or a contiguous copy."""
+    (m, k), h = x.shape, w_gate.shape[0]
+    ldx, xt, px = _operand(x, m, k, per, aligned)
+    ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
+    ldu, ut, pu = _operand(w_up, h, k, per, aligned)
+    if ldx is None or ldg is None or ldu is None or gt != ut:
+        # Neither rows nor columns contiguous, or weights stored in different ways.
+        x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+        ldx, xt, px = _operand(x, m, k, per, aligned)
+        ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
+        ldu, ut, pu = _operand(w_up, h, k, per, aligned)
+    ox = og = ou = 0
+    if px or pg or pu:
+        padded = [t for p, t in ((px, (x, k if xt else m, ldx, xt)),
+                                 (pg, (w_gate, k if gt else h, ldg, gt)),
+                                 (pu, (w_up, k if gt else h, ldu, gt))) if p]
+        buffer, offsets = _pack(padded, x, per, kind, index)
+        if px:
+            x, ox = buffer, offsets.pop(0)
+        if pg:
+            w_gate, og = buffer, offsets.pop(0)
+        if pu:
+            w_up, ou = buffer, offsets.pop(0)
+    return (x, ox, ldx, px), (w_gate, og, ldg, pg), (w_up, ou, ldu, pu), xt, gt
+
+
+def _matrix(operand, r: int, c: int, transposed: int) -> torch.Tensor:
+    """The (r, c) matrix that an operand of `_operands` holds."""
+    t, offset, ld, padded = operand
+    return t.as_strided((r, c), (1, ld) if transposed else (ld, 1), offset) if padded else t
 
 
 def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: bool):
@@ -253,27 +289,8 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
     # copy them; its few-rows kernel reads them at full speed.  The backward needs them aligned.
     aligned = kind != sdk.FP32 or keep or m > 32
     with _on_device(index):
-        ldx, xt, px = _operand(x, m, k, per, aligned)
-        ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
-        ldu, ut, pu = _operand(w_up, h, k, per, aligned)
-        if ldx is None or ldg is None or ldu is None or gt != ut:
-            # Neither rows nor columns contiguous, or weights stored in different ways.
-            x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
-            ldx, xt, px = _operand(x, m, k, per, aligned)
-            ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
-            ldu, ut, pu = _operand(w_up, h, k, per, aligned)
-        ox = og = ou = 0
-        if px or pg or pu:
-            padded = [t for p, t in ((px, (x, k if xt else m, ldx, xt)),
-                                     (pg, (w_gate, k if gt else h, ldg, gt)),
-                                     (pu, (w_up, k if gt else h, ldu, gt))) if p]
-            buffer, offsets = _pack(padded, x, per, kind, index)
-            if px:
-                x, ox = buffer, offsets.pop(0)
-            if pg:
-                w_gate, og = buffer, offsets.pop(0)
-            if pu:
-                w_up, ou = buffer, offsets.pop(0)
+        ops = _operands(x, w_gate, w_up, per, aligned, kind, index)
+        (xb, ox, ldx, _), (gb, og, ldg, _), (ub, ou, ldu, _), xt, wt = ops
         out = x.new_empty((m, h))
         pre, pg0, pu0, ldp = None, 0, 0, 0
         if keep:
@@ -282,8 +299,8 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
             pg0 = pre.data_ptr()
             pu0 = pg0 + m * ldp * 4
         size = 16 // per
-        d = Gated(_GATED_SIZE, kind, act, xt, gt, 0, m, h, k, x.data_ptr() + ox * size,
-                  w_gate.data_ptr() + og * size, w_up.data_ptr() + ou * size, ldx, ldg, ldu,
+        d = Gated(_GATED_SIZE, kind, act, xt, wt, 0, m, h, k, xb.data_ptr() + ox * size,
+                  gb.data_ptr() + og * size, ub.data_ptr() + ou * size, ldx, ldg, ldu,
                   0 if bias_gate is None else bias_gate.data_ptr(),
                   0 if bias_up is None else bias_up.data_ptr(), pg0, pu0, ldp, 0, 0,
                   _stream(index))
@@ -293,8 +310,8 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
             _check(st, "xvram_b200_gated_forward")
     if not keep:
         return out, None
-    return out, GatedSaved((x, w_gate, w_up, pre), (kind, act, xt, gt, m, h, k, ox, og, ou, ldx, ldg,
-                                                    ldu, ldp, dtype, device))
+    saved = (_matrix(ops[0], m, k, xt), _matrix(ops[1], h, k, wt), _matrix(ops[2], h, k, wt), pre)
+    return out, GatedSaved(saved, (kind, act, m, h, k, dtype, device))
 
 
 def _gated_workspace(d, backward: int, like: torch.Tensor):
@@ -319,12 +336,23 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     """Gradients (dx, dw_gate, dw_up, db_gate, db_up) of the block from dh = dL/dh; those that
     `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
     pre-activations are rounded to the type once, as the tensor cores' operands."""
-    kind, act, xt, wt, m, h, k, ox, og, ou, ldx, ldg, ldu, ldp, dtype, device = saved.layout
+    kind, act, m, h, k, dtype, device = saved.problem
     x, w_gate, w_up, pre = saved.tensors
+    # Strides are read from the tensors: autograd's saved-tensor hooks may have changed them.
+    ldp = (h + 3) // 4 * 4
+    for t, shape, of in ((x, (m, k), dtype), (w_gate, (h, k), dtype), (w_up, (h, k), dtype),
+                         (pre, (2, m, ldp), torch.float32)):
+        if t.shape != shape or t.dtype != of or t.device != device:
+            raise RuntimeError(f"a saved tensor of gated_linear must be {shape} {of} on {device} "
+                               f"(got {tuple(t.shape)} {t.dtype} on {t.device})")
     if dh.shape != (m, h) or dh.dtype != dtype or dh.device != device:
         raise ValueError(f"dh must be a ({m}, {h}) {dtype} tensor on {device}")
     index, size = device.index, 4 if kind == sdk.FP32 else 2
     with _on_device(index):
+        if not pre.is_contiguous() or pre.data_ptr() % 16:
+            pre = pre.clone(memory_format=torch.contiguous_format)
+        (x, ox, ldx, _), (w_gate, og, ldg, _), (w_up, ou, ldu, _), xt, wt = _operands(
+            x, w_gate, w_up, 16 // size, True, kind, index)
         dh, lddh = _rows(dh.detach() if dh.requires_grad else dh)
         dx = dh.new_empty((m, k)) if needs[0] else None
         dwg = dh.new_empty((h, k)) if needs[1] else None
@@ -347,14 +375,14 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
         out, saved = _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
         ctx.save_for_backward(*saved.tensors)
-        ctx.layout = saved.layout
+        ctx.problem = saved.problem
         return out
 
     @staticmethod
     def backward(ctx, dh):
         if torch.is_grad_enabled():  # create_graph=True
             raise RuntimeError("gated_linear has no second derivative")
-        saved = GatedSaved(ctx.saved_tensors, ctx.layout)
+        saved = GatedSaved(ctx.saved_tensors, ctx.problem)
         return (*gated_linear_backward(dh, saved, ctx.needs_input_grad), None)
 
 
