@@ -40,6 +40,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import device as xd
 from . import sdk
@@ -158,6 +159,15 @@ _stream = torch._C._cuda_getCurrentRawStream if hasattr(
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def _refuse_tangents(what: str, *tensors) -> None:
+    """Forward-mode derivatives are not implemented, and a result without a tangent would read
+    as a zero derivative.  Outside a dual level no tensor has a tangent."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+            for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _operand(x: torch.Tensor, r: int, c: int, per: int, aligned: bool):
@@ -327,6 +337,7 @@ def _gated_workspace(d, backward: int, like: torch.Tensor):
 def gated_linear_forward(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu"):
     """(h, saved): the gated block's result and what `gated_linear_backward` needs.  For callers
     that drive the backward pass themselves; autograd is not involved."""
+    _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     with torch.no_grad():
         return _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
 
@@ -336,6 +347,7 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     """Gradients (dx, dw_gate, dw_up, db_gate, db_up) of the block from dh = dL/dh; those that
     `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
     pre-activations are rounded to the type once, as the tensor cores' operands."""
+    _refuse_tangents("gated_linear's backward", dh)
     kind, act, m, h, k, dtype, device = saved.problem
     x, w_gate, w_up, pre = saved.tensors
     # Strides are read from the tensors: autograd's saved-tensor hooks may have changed them.
@@ -394,7 +406,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     gelu, gelu_tanh, relu or sigmoid.  float16 / bfloat16 run as one tensor-core kernel with FP32
     accumulation and one rounding, float32 in strict FP32.  Row-major and transposed operands
     are read in place (16-bit ones where their base and leading dimension are multiples of 16
-    bytes; others are copied first).  Differentiable once in every tensor argument."""
+    bytes; others are copied first).  Differentiable once in every tensor argument, in reverse
+    mode; tensors with a forward-mode tangent are refused."""
+    _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     if torch.is_grad_enabled() and (
             x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
             (bias_gate is not None and bias_gate.requires_grad) or
@@ -448,6 +462,7 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
         raise TypeError(f"quantize_mxfp4 takes float16, bfloat16 or float32 (got {x.dtype})")
     if x.dim() != 2:
         raise ValueError("expected a 2-D tensor")
+    _refuse_tangents("quantize_mxfp4", x)
     if x.device.type != "cuda":
         raise RuntimeError("quantize_mxfp4 needs a CUDA tensor (there is no CPU path)")
     if torch.is_grad_enabled() and x.requires_grad:
@@ -499,6 +514,7 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
     n = first.shape[0]
     if k == 0:
         raise ValueError(f"{what} needs at least one input feature")
+    _refuse_tangents(what, x, *biases)
     if device.type != "cuda" or first.codes.device != device or last.codes.device != device:
         raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
     if torch.is_grad_enabled() and (
