@@ -174,17 +174,21 @@ def _operand(x: torch.Tensor, r: int, c: int, per: int, aligned: bool):
     """(leading dimension, transposed, padded) of x as the kernels read it.  padded: x must be
     copied with rows (or, transposed, columns) of whole 16 bytes first.  `per`: elements in 16
     bytes; `aligned`: rows must be multiples of them.  (None, ...): neither rows nor columns are
-    contiguous."""
+    contiguous, which a contiguous x never answers."""
     s0, s1 = x.stride()
+    # Strides of empty tensors and of sizes of one are never used, and torch leaves them as they
+    # are, in what it calls contiguous too.
+    if r == 0:
+        return (c + per - 1) // per * per, 0, False
+    if c == 1:
+        s1 = 1
     if s1 == 1 and (s0 >= c or r == 1):
-        if r == 1:  # one row's stride is never used
+        if r == 1:
             s0 = (c + per - 1) // per * per
         if not aligned or (s0 % per == 0 and x.data_ptr() % 16 == 0):
             return s0, 0, False
         return (c + per - 1) // per * per, 0, True
-    if s0 == 1 and (s1 >= r or c == 1):
-        if c == 1:
-            s1 = (r + per - 1) // per * per
+    if s0 == 1 and s1 >= r:
         if not aligned or (s1 % per == 0 and x.data_ptr() % 16 == 0):
             return s1, 1, False
         return (r + per - 1) // per * per, 1, True
