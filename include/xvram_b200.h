@@ -392,7 +392,9 @@ enum {
  * Storage: a row's k values contiguous, leading dimensions in elements between rows (the
  * column-major k x rows matrix); x_transposed / w_transposed = 1 for operands stored the
  * other way (k rows of m or h values).  FP16 / BF16 operands need 16-byte aligned bases and
- * leading dimensions that are multiples of 8; FP32 operands any.  Biases (0 for none) hold h
+ * leading dimensions that are multiples of 8; FP32 operands any.  The forward takes FP16 / BF16
+ * operands from any element on too, when none is transposed, for one row, and for up to 4 rows
+ * while h x k is at most 2^23.  Biases (0 for none) hold h
  * values of the data type.  pre_gate and pre_up, both or neither, receive x Wg^T + bg and
  * x Wu^T + bu in FP32 (m x h, ld_pre a multiple of 4, 16-byte aligned) for the backward pass.
  * The workspace (256-byte aligned, xvram_b200_gated_workspace_bytes) may be reused once the

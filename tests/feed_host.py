@@ -43,10 +43,13 @@ class HostLibrary:
     def __init__(self):
         self.calls = []
 
-    def _operands(self, d):
+    def _operands(self, d, backward):
         per = 16 // TYPES[d.data_type]().itemsize
+        # The kernel for few rows reads any element-aligned row.
+        few = not d.x_transposed and not d.w_transposed and (
+            d.m == 1 or (d.m <= 4 and d.h * d.k <= 1 << 23))
         for p, ld in ((d.x, d.ldx), (d.w_gate, d.ld_gate), (d.w_up, d.ld_up)):
-            if d.data_type != 2 and (p % 16 or ld % per):
+            if d.data_type != 2 and (backward or not few) and (p % 16 or ld % per):
                 return None
         return (matrix(d.x, d.m, d.k, d.ldx, d.data_type, d.x_transposed).astype(np.float64),
                 *(matrix(p, d.h, d.k, ld, d.data_type, d.w_transposed).astype(np.float64)
@@ -60,7 +63,7 @@ class HostLibrary:
         self.calls.append("forward")
         if d.m == 0 or d.h == 0:
             return 0
-        if (ops := self._operands(d)) is None:
+        if (ops := self._operands(d, False)) is None:
             return 1
         x, wg, wu = ops
         g, u = x @ wg.T, x @ wu.T
@@ -81,7 +84,7 @@ class HostLibrary:
         self.calls.append("backward")
         if d.m == 0 or d.h == 0:
             return 0
-        if (ops := self._operands(d)) is None:
+        if (ops := self._operands(d, True)) is None:
             return 1
         x, wg, wu = ops
         g, u = (matrix(p, d.m, d.h, d.ld_pre, 2).astype(np.float64) for p in (d.pre_gate, d.pre_up))

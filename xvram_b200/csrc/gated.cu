@@ -429,7 +429,7 @@ bool few_rows(const GatedProblem& q) {
   if (q.x_transposed || q.w_transposed)
     return false;
   if (q.type != GatedType::f32)
-    return q.m == 1 || (q.m <= 4 && static_cast<long long>(q.h) * q.k <= 8 << 20);
+    return q.m == 1 || (q.m <= 4 && static_cast<long long>(q.h) * q.k <= 1 << 23);
   if (q.m > 512)
     return false;
   const long long tiles = ((q.h + 127ll) / 128) * ((q.m + 127) / 128), sms = tc::sm_count();

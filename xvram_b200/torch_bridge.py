@@ -253,10 +253,15 @@ class GatedSaved:
         self.tensors, self.problem = tensors, problem
 
 
-def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int):
+# Up to _FEW_ROWS rows of 16-bit values run on the forward's few-rows kernel, which reads rows from
+# any element on, while a weight has at most _FEW_VALUES values; one row always does.
+_FEW_ROWS, _FEW_VALUES = 4, 1 << 23
+
+
+def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int, few: bool = False):
     """x and the weights as the kernels read them: three (buffer, element offset, leading
     dimension, padded) and whether x and the weights are transposed.  Not padded: the buffer is
-    the tensor itself or a contiguous copy."""
+    the tensor itself or a contiguous copy.  `few`: the few-rows kernel may take the operands."""
     (m, k), h = x.shape, w_gate.shape[0]
     ldx, xt, px = _operand(x, m, k, per, aligned)
     ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
@@ -267,6 +272,12 @@ def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int):
         ldx, xt, px = _operand(x, m, k, per, aligned)
         ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
         ldu, ut, pu = _operand(w_up, h, k, per, aligned)
+    if few and (pg or pu) and not xt and not gt:
+        # Copying the weights costs more than reading them by elements (BF16, 1 x 2047 x 4099: 22.1
+        # us against 13.7, 1 x 4095 x 8192 76 against 36, 4 x 1001 x 2730 13.6 against 8.6); copying x
+        # alone does not.
+        (ldx, _, px), (ldg, _, pg), (ldu, _, pu) = (
+            _operand(t, t.shape[0], k, per, False) for t in (x, w_gate, w_up))
     ox = og = ou = 0
     if px or pg or pu:
         padded = [t for p, t in ((px, (x, k if xt else m, ldx, xt)),
@@ -302,8 +313,9 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
     # The float32 GEMM reads any operand, but unaligned ones several times slower than it takes to
     # copy them; its few-rows kernel reads them at full speed.  The backward needs them aligned.
     aligned = kind != sdk.FP32 or keep or m > 32
+    few = kind != sdk.FP32 and not keep and (m == 1 or (m <= _FEW_ROWS and h * k <= _FEW_VALUES))
     with _on_device(index):
-        ops = _operands(x, w_gate, w_up, per, aligned, kind, index)
+        ops = _operands(x, w_gate, w_up, per, aligned, kind, index, few)
         (xb, ox, ldx, _), (gb, og, ldg, _), (ub, ou, ldu, _), xt, wt = ops
         out = x.new_empty((m, h))
         pre, pg0, pu0, ldp = None, 0, 0, 0
@@ -410,7 +422,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     gelu, gelu_tanh, relu or sigmoid.  float16 / bfloat16 run as one tensor-core kernel with FP32
     accumulation and one rounding, float32 in strict FP32.  Row-major and transposed operands
     are read in place (16-bit ones where their base and leading dimension are multiples of 16
-    bytes; others are copied first).  Differentiable once in every tensor argument, in reverse
+    bytes; others are copied first, unless there are up to four rows).  Differentiable once in every tensor argument, in reverse
     mode; tensors with a forward-mode tangent are refused."""
     _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     if torch.is_grad_enabled() and (
