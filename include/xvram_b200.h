@@ -481,7 +481,8 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
  * once the call's work on `stream` is done); up to XVRAM_B200_MXFP4_DIRECT_ROWS rows of at most
  * XVRAM_B200_MXFP4_DIRECT_VALUES values together are quantised inside the product instead, and
  * x_codes and x_scales are not used (0 allowed).  With x = 0, x_codes and x_scales as they are.  Biases (0 for
- * none) hold n values of out_type.
+ * none) hold n values of out_type.  XVRAM_STATUS_UNSUPPORTED: quantised inside the product, a row this
+ * long needs larger clusters than the device runs; quantise it first.
  */
 #define XVRAM_B200_MXFP4_DIRECT_ROWS 16
 #define XVRAM_B200_MXFP4_DIRECT_VALUES 65536

@@ -20,6 +20,7 @@
 #pragma once
 
 #include "mxfp4_block.cuh"
+#include "split_rule.hpp"
 
 #include <algorithm>
 
@@ -372,76 +373,49 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Rows of A that a stage holds.
 inline int split_rows(int m) { return std::min(128, (m + 7) / 8 * 8); }
 
-// CTAs of clusters of `size` (one CTA per SM) that the current device runs at once.
-template <class F>
-long long cluster_capacity(F* kernel, int size, long long sms) {
-  static std::atomic<int> known[64][4]; // by device and log2(size)
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64)
-    return 0;
-  std::atomic<int>& slot = known[dev][size == 2 ? 1 : size == 4 ? 2 : 3];
-  int clusters = slot.load(std::memory_order_relaxed);
-  if (clusters == 0) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = size;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(sms / size * size));
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kSplitSmem;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess) {
-      cudaGetLastError();
-      clusters = 0;
-    }
-    clusters = std::max(clusters, 0) + 1; // 0: not asked yet
-    slot.store(clusters, std::memory_order_relaxed);
-  }
-  return static_cast<long long>(clusters - 1) * size;
-}
-
 template <Kind K, Epilogue E, class T>
 cudaError_t allow_split() {
   static std::atomic<uint64_t> done{0};
   return tc::allow_smem(feed_split_kernel<K, E, T>, kSplitSmem, done);
 }
 
-// The cluster size with the least estimated time, and that time in us: a stage takes 0.75 when all SMs
-// read from HBM and at least 0.45 (one SM's rate); a wave of CTAs 2.5 to start, joining 1.  Clusters
-// fit an SM count that the hardware's grouping of SMs limits.  A quantised A (a_bytes per stage)
-// has to fit, whatever the time; 0 splits if it does not.
-struct Split {
-  int splits;
-  double us;
-};
+// The rule's answer for this kernel on the current device (split_rule.hpp).  a_bytes: a quantised
+// A's per stage, 0 when A streams.  Clusters of one CTA per SM; each kernel has its own table.
 template <Kind K, Epilogue E, class T>
-Split choose_split(const Params& p, int a_bytes) {
+cudaError_t choose_split(const Params& p, int a_bytes, Split* best) {
   constexpr int kTileN = E == Epilogue::gated ? 128 : 256;
-  const auto kernel = feed_split_kernel<K, E, T>;
+  static CapacityTable table;
   const long long tiles =
       static_cast<long long>((p.m + 127) / 128) * ((p.n + kTileN - 1) / kTileN);
   const long long sms = tc::sm_count();
-  Split best{0, 0};
-  if (allow_split<K, E, T>() != cudaSuccess) // the capacity query needs it too
-    return best;
-  for (int s = 1; s <= 8 && s <= p.k_tiles; s *= 2) {
-    const long long ctas = tiles * s, cap = s == 1 ? sms : cluster_capacity(kernel, s, sms);
-    if (cap < s)
-      continue;
-    const double stage_us =
-        std::max(0.45, 0.75 * static_cast<double>(std::min(ctas, cap)) / static_cast<double>(sms));
-    const double t = static_cast<double>((ctas + cap - 1) / cap) *
-                         (2.5 + stage_us * ((p.k_tiles + s - 1) / s)) +
-                     (s > 1 ? 1.0 : 0.0);
-    const bool fits = !a_bytes || ((p.k_tiles + s - 1) / s) *
-                                          (a_bytes + static_cast<int>(kScaleTile)) <=
-                                      kDirectBytes;
-    if (fits && (best.splits == 0 || t < best.us))
-      best = {s, t};
-  }
-  return best;
+  *best = Split{};
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess)
+    return e;
+  if (cudaError_t e = allow_split<K, E, T>(); e != cudaSuccess) // the capacity query needs it too
+    return e;
+  const auto capacity = [&](int size, long long* ctas) {
+    return table.ctas(dev, size, ctas, [&](int* clusters) {
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = size;
+      attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(static_cast<unsigned>(sms / size * size));
+      config.blockDim = dim3(kThreads);
+      config.dynamicSmemBytes = kSplitSmem;
+      config.attrs = &attr;
+      config.numAttrs = 1;
+      const cudaError_t e =
+          cudaOccupancyMaxActiveClusters(clusters, feed_split_kernel<K, E, T>, &config);
+      if (e != cudaSuccess)
+        cudaGetLastError();
+      return static_cast<int>(e);
+    });
+  };
+  return static_cast<cudaError_t>(cheapest_split(
+      tiles, p.k_tiles, sms, a_bytes ? a_bytes + static_cast<int>(kScaleTile) : 0, kDirectBytes,
+      capacity, best));
 }
 
 // `after`: launched behind a kernel of the same stream that allows programmatic overlap.
@@ -458,9 +432,12 @@ cudaError_t launch_split(const Maps& maps, const Params& p, const DirectInput& i
   const bool direct = in.x != nullptr;
   q.a_bytes = K == Kind::f16 && p.a_mn ? kPart : split_rows(p.m) * 128;
   q.p.tiles_m = (p.m + 127) / 128;
-  q.splits = choose_split<K, E, T>(p, direct ? q.a_bytes : 0).splits;
+  Split split;
+  if (cudaError_t e = choose_split<K, E, T>(p, direct ? q.a_bytes : 0, &split); e != cudaSuccess)
+    return e;
+  q.splits = split.splits;
   if (q.splits == 0)
-    return cudaErrorInvalidValue;
+    return cudaErrorNotSupported; // this device's clusters are too small for the quantised rows
   const int most = (p.k_tiles + q.splits - 1) / q.splits; // stages of a CTA
   q.ring = direct ? most * (q.a_bytes + static_cast<int>(kScaleTile)) : 0;
   const int stage = (direct ? 0 : q.a_bytes) + 2 * kPart +

@@ -313,9 +313,11 @@ cudaError_t backward_16(const GatedProblem& q, const GatedGradients& d, char* ws
     const long long pairs = tc::sm_count() / 2;
     const long long waves =
         (static_cast<long long>(p.tiles_n) * ((q.m + 255) / 256) + pairs - 1) / pairs;
-    cudaError_t e;
-    if (q.m <= 128 || choose_split<Kind::f16, Epilogue::plain, T>(p, 0).us <
-                          static_cast<double>(waves) * (3.0 + 0.3 * p.k_tiles)) {
+    Split split;
+    cudaError_t e = choose_split<Kind::f16, Epilogue::plain, T>(p, 0, &split);
+    if (e != cudaSuccess)
+      return e;
+    if (q.m <= 128 || split.us < static_cast<double>(waves) * (3.0 + 0.3 * p.k_tiles)) {
       p.idesc = idesc_f16(bf16, p.a_mn, p.b_mn, 128, 256);
       e = launch_split<Kind::f16, Epilogue::plain, T>(maps, p, DirectInput{}, false, stream);
     } else {

@@ -31,6 +31,8 @@ xvram_status from_cuda(cudaError_t e) {
     return XVRAM_STATUS_INVALID_ARGUMENT;
   case cudaErrorMemoryAllocation:
     return XVRAM_STATUS_DEVICE_OUT_OF_MEMORY;
+  case cudaErrorNotSupported:
+    return XVRAM_STATUS_UNSUPPORTED;
   case cudaErrorNoDevice:
   case cudaErrorInsufficientDriver:
     return XVRAM_STATUS_UNAVAILABLE;
