@@ -479,8 +479,9 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
  * x (m x k): with x set, rows of `x_type` values, ldx elements apart, which are quantised into
  * x_codes and x_scales first (caller's memory, as xvram_b200_mxfp4_bytes says; it may be reused
  * once the call's work on `stream` is done); up to XVRAM_B200_MXFP4_DIRECT_ROWS rows of at most
- * XVRAM_B200_MXFP4_DIRECT_VALUES values together are quantised inside the product instead, and
- * x_codes and x_scales are not used (0 allowed).  With x = 0, x_codes and x_scales as they are.  Biases (0 for
+ * XVRAM_B200_MXFP4_DIRECT_VALUES values together can be quantised inside the product instead:
+ * with x_codes and x_scales 0 they are, and with that memory given where it is faster (from
+ * about half of these values on it seldom is).  With x = 0, x_codes and x_scales as they are.  Biases (0 for
  * none) hold n values of out_type.  XVRAM_STATUS_UNSUPPORTED: quantised inside the product, a row this
  * long needs larger clusters than the device runs; quantise it first.
  */

@@ -155,8 +155,8 @@ struct Mxfp4Operand {
   unsigned char *codes = nullptr, *scales = nullptr;
 };
 // out = a b[0]^T (+ bias[0], ReLU), or with b[1] act(a b[0]^T + bias[0]) * (a b[1]^T + bias[1]);
-// out and the biases are of `type`.  With x set, x is quantised into a first, or, when
-// mxfp4_direct says so, inside the product, which then does not touch a.
+// out and the biases are of `type`.  With x set, x is quantised into a first, or, few values of it,
+// inside the product, which then does not touch a; a may be empty where that is possible.
 struct Mxfp4Product {
   GatedType x_type = GatedType::f32;
   const void* x = nullptr;
@@ -174,7 +174,6 @@ cudaError_t mxfp4_quantize(GatedType type, const void* src, long long lds, int r
 cudaError_t mxfp4_dequantize(GatedType type, const unsigned char* codes,
                              const unsigned char* scales, int rows, int cols, void* dst,
                              long long ldd, cudaStream_t stream);
-bool mxfp4_direct(const Mxfp4Product& q);
 cudaError_t mxfp4_product(const Mxfp4Product& q, cudaStream_t stream);
 cudaError_t read_and_clear_kernel_error_mxfp4(unsigned int* out, cudaStream_t stream);
 

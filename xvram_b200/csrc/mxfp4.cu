@@ -187,12 +187,56 @@ bool operand_maps(CUtensorMap* codes, CUtensorMap* scales, const Mxfp4Operand& o
                         (static_cast<uint64_t>(rows) + 127) / 128, tiles * 512, 256, 1, false);
 }
 
+// Few input values can be quantised by the product itself: each CTA brings its K range of them into
+// its shared memory while its first weights arrive.  That saves the pass in front, but each
+// cluster quantises its rows again, before its first MMA: it pays up to about 16384 values per
+// CTA.  Device time of calls in a graph and, in brackets, of calls in a row from Python, direct against
+// a pass in front:
+//   values per CTA  8192 (4 x 4096 x 8192 gated)    14.0 us (16.5) against 14.3 (16.9)
+//                   8192 (1 x 65536 x 1024 linear)  23.6 us (25.8) against 26.6 (28.9)
+//                  16384 (8 x 4096 x 8192 gated)    14.9 us (16.6) against 14.3 (16.9)
+//                  16384 (16 x 2048 x 8192 gated)   11.6 us (14.2) against 10.7 (17.3)
+//                  24576 (12 x 4096 x 8192 gated)   16.0 us (18.6) against 14.1 (16.9)
+//                  32768 (16 x 4096 x 8192 gated)   16.9 us (18.6) against 14.1 (16.9)
+static_assert(kDirectRows == XVRAM_B200_MXFP4_DIRECT_ROWS &&
+                  kDirectValues == XVRAM_B200_MXFP4_DIRECT_VALUES,
+              "the header says the same");
+constexpr long long kDirectShare = 16384;
+
 template <Epilogue E, class T>
-cudaError_t product(const Mxfp4Product& q, bool after, cudaStream_t stream) {
+cudaError_t choose_direct(const Mxfp4Product& q, const Params& p, bool* direct) {
+  *direct = q.x && q.m <= kDirectRows && static_cast<long long>(q.m) * q.k <= kDirectValues;
+  if (!*direct || !q.a.codes) // without memory for the codes there is no choice
+    return cudaSuccess;
+  Split split;
+  if (cudaError_t e = choose_split<Kind::mxf4, E, T>(p, split_rows(q.m) * 128, &split);
+      e != cudaSuccess)
+    return e;
+  *direct = split.splits > 0 &&
+            static_cast<long long>(q.m) *
+                    std::min<long long>(q.k, (p.k_tiles + split.splits - 1) / split.splits * 256ll) <=
+                kDirectShare;
+  return cudaSuccess;
+}
+
+template <Epilogue E, class T>
+cudaError_t product(const Mxfp4Product& q, cudaStream_t stream) {
   constexpr bool gated = E == Epilogue::gated;
   constexpr int kTileN = gated ? 128 : 256;
   const int blocks = (q.k + kBlock - 1) / kBlock;
-  const bool split = q.m <= 128, direct = mxfp4_direct(q);
+  const bool split = q.m <= 128;
+  Params p{};
+  p.m = q.m;
+  p.n = q.n;
+  p.k_tiles = p.k_split = (blocks + 7) / 8;
+  bool direct;
+  if (cudaError_t e = choose_direct<E, T>(q, p, &direct); e != cudaSuccess)
+    return e;
+  const bool after = q.x && !direct;
+  if (after)
+    if (cudaError_t e = mxfp4_quantize(q.x_type, q.x, q.ldx, q.m, q.k, q.a.codes, q.a.scales, stream);
+        e != cudaSuccess)
+      return e;
   Maps maps{};
   if (!direct &&
       !operand_maps(&maps.a[0], &maps.scale_a, q.a, q.m, blocks, split ? split_rows(q.m) : 128))
@@ -201,10 +245,6 @@ cudaError_t product(const Mxfp4Product& q, bool after, cudaStream_t stream) {
     if (!operand_maps(&maps.b[i], &maps.scale_b[i], q.b[gated ? i : 0], q.n, blocks, 128))
       return cudaErrorInvalidValue;
   maps.a[1] = maps.a[0];
-  Params p{};
-  p.m = q.m;
-  p.n = q.n;
-  p.k_tiles = p.k_split = (blocks + 7) / 8;
   p.tiles_n = (q.n + kTileN - 1) / kTileN;
   p.batches = 1;
   p.act = q.act;
@@ -252,35 +292,18 @@ cudaError_t mxfp4_dequantize(GatedType type, const unsigned char* codes,
   }
 }
 
-// Few input values are quantised by the product itself: each CTA brings its K range of them into
-// its shared memory while its first weights arrive.  4096 x 8192, device time and, in brackets,
-// a call from Python: one row 12.6 us (10.5) against 13.5 (16) with the pass in front, 16 rows 15.8
-// (17.6) against 13.4 (19.5).
-static_assert(kDirectRows == XVRAM_B200_MXFP4_DIRECT_ROWS &&
-                  kDirectValues == XVRAM_B200_MXFP4_DIRECT_VALUES,
-              "the header says the same");
-bool mxfp4_direct(const Mxfp4Product& q) {
-  return q.x && q.m <= kDirectRows &&
-         static_cast<long long>(q.m) * q.k <= kDirectValues;
-}
-
 cudaError_t mxfp4_product(const Mxfp4Product& q, cudaStream_t stream) {
-  const bool after = q.x && !mxfp4_direct(q);
-  if (after)
-    if (cudaError_t e = mxfp4_quantize(q.x_type, q.x, q.ldx, q.m, q.k, q.a.codes, q.a.scales, stream);
-        e != cudaSuccess)
-      return e;
   if (q.b[1].codes) {
     switch (q.type) {
-    case GatedType::f16: return product<Epilogue::gated, __half>(q, after, stream);
-    case GatedType::bf16: return product<Epilogue::gated, __nv_bfloat16>(q, after, stream);
-    default: return product<Epilogue::gated, float>(q, after, stream);
+    case GatedType::f16: return product<Epilogue::gated, __half>(q, stream);
+    case GatedType::bf16: return product<Epilogue::gated, __nv_bfloat16>(q, stream);
+    default: return product<Epilogue::gated, float>(q, stream);
     }
   }
   switch (q.type) {
-  case GatedType::f16: return product<Epilogue::plain, __half>(q, after, stream);
-  case GatedType::bf16: return product<Epilogue::plain, __nv_bfloat16>(q, after, stream);
-  default: return product<Epilogue::plain, float>(q, after, stream);
+  case GatedType::f16: return product<Epilogue::plain, __half>(q, stream);
+  case GatedType::bf16: return product<Epilogue::plain, __nv_bfloat16>(q, stream);
+  default: return product<Epilogue::plain, float>(q, stream);
   }
 }
 

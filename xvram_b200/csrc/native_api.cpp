@@ -194,7 +194,8 @@ xvram_status run_mxfp4(const xvram_b200_mxfp4_product_v1& d, bool gated) {
   q.k = static_cast<int>(d.k);
   q.act = static_cast<int>(d.activation);
   q.relu = !gated && d.activation == XVRAM_B200_ACTIVATION_RELU;
-  q.a = {bytes(d.x_codes), bytes(d.x_scales)};
+  if (mxfp4_operand(d.x_codes, d.x_scales))
+    q.a = {bytes(d.x_codes), bytes(d.x_scales)};
   q.out = pointer(d.out);
   q.ldo = d.ld_out;
   return from_cuda(mxfp4_product(q, as_stream(d.stream)));
