@@ -443,8 +443,8 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_forward(const xvram_b200
  * set; each of dx (m x k), dw_gate and dw_up (h x k, ld_dw), db_gate and db_up (h) may be 0 when
  * it is not wanted.  Gradients have the data type and are stored with contiguous rows whatever
  * the operands' transposition.  For FP16 / BF16 the gradients of the pre-activations are rounded
- * to the data type once, as the tensor cores' operands; all sums are FP32.  Results do not depend
- * on timing.  With m = 0 the weights' and biases' gradients are zeros. */
+ * to the data type once, as the tensor cores' operands (FP16: times a power of two, where its range
+ * would lose them); all sums are FP32.  Results do not depend on timing.  With m = 0 the weights' and biases' gradients are zeros. */
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_backward(
     const xvram_b200_gated_v1* problem, uint64_t dout, int64_t ld_dout, uint64_t dx, int64_t ld_dx,
     uint64_t dw_gate, uint64_t dw_up, int64_t ld_dw, uint64_t db_gate, uint64_t db_up);

@@ -22,6 +22,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace xvram::feed {
 
 constexpr int kThreads = 320; // producer, MMA, 8 epilogue warps
@@ -53,6 +55,7 @@ struct Params {
   int tiles_m, tiles_n, batches;
   int a_mn, b_mn;         // 16-bit operands stored M-/N-major
   int act, relu;
+  const unsigned* top;    // FP16, plain: the A operands hold their values times fp16_scale(*top); 0: once
   int unit;               // widest access the output rows allow, in bytes (store_unit)
   uint32_t idesc;
   const void *bias0, *bias1;
@@ -62,6 +65,21 @@ struct Params {
   long long lds;
   unsigned long long timeout_ns;
 };
+
+// FP16's range.  dg and du are FP16 operands of products whose results may fit where they do not, so
+// they are held times a power of two when their largest finite magnitude (`top`, a float's bits) is
+// above FP16's 65504, or below 2^-8, where FP16's smallest step of 2^-24 would be more than 2^-16 of
+// it.  It then lies in [2^14, 2^15), and the products' results are multiplied by the inverse,
+// exactly.
+__device__ __forceinline__ float fp16_scale(unsigned top) {
+  if (top == 0 || (top >= 0x3b800000u && top <= 0x477fe000u)) // 2^-8, 65504
+    return 1.0f;
+  const int e = min(141 + 127 - static_cast<int>(top >> 23), 227); // 14 - floor(log2 top), at most 100
+  return __uint_as_float(static_cast<unsigned>(e) << 23);
+}
+__device__ __forceinline__ float fp16_unscale(const unsigned* top) {
+  return top ? __uint_as_float((254u << 23) - __float_as_uint(fp16_scale(*top))) : 1.0f;
+}
 
 // Instruction descriptors.  16-bit: D F32, operand format (0 FP16, 1 BF16), majors, N and M.
 inline uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn, int m, int n) {
@@ -426,11 +444,11 @@ __device__ __forceinline__ void add_bias_chunk(const void* bias, int col, int n,
 
 // A warp's share of an accumulator (TMEM lanes of t_row) to results: the gated form's 64 outputs
 // or the plain form's 128 columns of column half `half`, of rows row0.. and columns from `col` on.
-// `release` is called once the accumulator has been read.  Collective over the warp; T is a
-// 16-bit type.
+// `release` is called once the accumulator has been read.  `unscale` is fp16_unscale's for the plain
+// form.  Collective over the warp; T is a 16-bit type.
 template <Epilogue E, class T, class F>
 __device__ __forceinline__ void finish_unit(const Params& p, uint32_t t_row, int half, int row0,
-                                            int col, T* out, unsigned char* block,
+                                            int col, T* out, unsigned char* block, float unscale,
                                             const F& release) {
   static_assert(sizeof(T) == 2, "two chunks fill a block row");
   constexpr int kChunks = E == Epilogue::gated ? 4 : 8;
@@ -453,6 +471,11 @@ __device__ __forceinline__ void finish_unit(const Params& p, uint32_t t_row, int
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         v[i] = __uint_as_float(r0[i]);
+      if constexpr (E == Epilogue::plain && std::is_same_v<T, __half>) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[i] *= unscale;
+      }
       add_bias_chunk<T>(p.bias0, cc, p.n, v);
       if constexpr (E == Epilogue::gated) {
         float w[16];

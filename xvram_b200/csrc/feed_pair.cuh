@@ -250,6 +250,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<K, HALVES>
     const uint32_t release = tc::cluster_addr(smem_u32(acc_empty), 0) + 8 * group;
     int unit = 0;
     bool stop = false;
+    float unscale = 1.0f;
+    if constexpr (K == Kind::f16 && E == Epilogue::plain && std::is_same_v<T, __half>)
+      unscale = fp16_unscale(p.top);
     for (int t = first; t < tiles && !stop; t += pairs) {
       int batch, m0, n0;
       tile_origin(p, t, 256 * HALVES, kTileN, batch, m0, n0);
@@ -285,7 +288,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairShape<K, HALVES>
           finish_rows<E, T>(p, r, row0, col, out, blocks + (warp - 2) * kStageBlock);
         } else {
           finish_unit<E, T>(p, t_row, half, row0, col, out, blocks + (warp - 2) * kSubBlock,
-                            hand_back);
+                            unscale, hand_back);
         }
       }
     }

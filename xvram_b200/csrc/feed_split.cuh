@@ -316,6 +316,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int groups = cols / 4;
   T* out = static_cast<T*>(p.out[0]) + m0 * p.ldo;
   const long long kept = m0 * p.lds;
+  float unscale = 1.0f;
+  if constexpr (K == Kind::f16 && E == Epilogue::plain && std::is_same_v<T, __half>)
+    unscale = fp16_unscale(p.top);
   for (int i = tid; i < rows * groups; i += kThreads) {
     const int r = i / groups, c = rank * cols + (i - r * groups) * 4;
     const int col = n0 + c;
@@ -331,6 +334,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4 y = load_cluster(from + 128 * 4);
         w[0] += y.x, w[1] += y.y, w[2] += y.z, w[3] += y.w;
       }
+    }
+    if constexpr (K == Kind::f16 && E == Epilogue::plain && std::is_same_v<T, __half>) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[j] *= unscale;
     }
     add_bias<T>(p.bias0, col, p.n, v);
     if constexpr (E == Epilogue::gated) {

@@ -365,7 +365,8 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
                           needs=(True, True, True, True, True)):
     """Gradients (dx, dw_gate, dw_up, db_gate, db_up) of the block from dh = dL/dh; those that
     `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
-    pre-activations are rounded to the type once, as the tensor cores' operands."""
+    pre-activations are rounded to the type once, as the tensor cores' operands (float16: times a
+    power of two where its range would lose them, so that gradients which fit are right)."""
     _refuse_tangents("gated_linear's backward", dh)
     kind, act, m, h, k, dtype, device = saved.problem
     x, w_gate, w_up, pre = saved.tensors
