@@ -226,7 +226,7 @@ _PRODUCT_SIZE = ctypes.sizeof(Mxfp4Product)
 def _check_bias(b: torch.Tensor, h: int, dtype: torch.dtype, device: torch.device, name: str):
     if b.dtype != dtype or b.device != device or b.dim() != 1 or b.numel() != h:
         raise ValueError(f"{name} must hold {h} values of the result's type on its device")
-    return b.contiguous()
+    return (b.resolve_neg() if h == 1 else b).contiguous()
 
 
 def _check_gated(x, w_gate, w_up, dtype: torch.dtype, device: torch.device) -> None:
@@ -266,6 +266,10 @@ def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int, f
     dimension, padded) and whether x and the weights are transposed.  Not padded: the buffer is
     the tensor itself or a contiguous copy.  `few`: the few-rows kernel may take the operands."""
     (m, k), h = x.shape, w_gate.shape[0]
+    if k == 1:
+        # The imaginary part of a conjugate stands for its memory's negative.  Its elements are
+        # never neighbours, so that it is copied below unless the stride does not count.
+        x, w_gate, w_up = x.resolve_neg(), w_gate.resolve_neg(), w_up.resolve_neg()
     ldx, xt, px = _operand(x, m, k, per, aligned)
     ldg, gt, pg = _operand(w_gate, h, k, per, aligned)
     ldu, ut, pu = _operand(w_up, h, k, per, aligned)
@@ -466,8 +470,10 @@ class Mxfp4Matrix:
 
 def _rows(x: torch.Tensor):
     """(x with contiguous rows, its leading dimension)"""
-    s0, s1 = x.stride()
     cols = x.shape[1]
+    if cols == 1:
+        x = x.resolve_neg()
+    s0, s1 = x.stride()
     if s1 != 1 or s0 < cols:
         x = x.contiguous()
         s0 = cols
