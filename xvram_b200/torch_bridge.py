@@ -161,12 +161,16 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _dual_level() -> bool:
+    """Whether a forward-mode level is open.  Outside one no tensor has a tangent."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def _refuse_tangents(what: str, *tensors) -> None:
     """Forward-mode derivatives are not implemented, and a result without a tangent would read
-    as a zero derivative.  Outside a dual level no tensor has a tangent."""
-    if getattr(forward_ad, "_current_level", 0) >= 0 and any(
-            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
-            for t in tensors):
+    as a zero derivative."""
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+           for t in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
@@ -247,13 +251,14 @@ def _check_gated(x, w_gate, w_up, dtype: torch.dtype, device: torch.device) -> N
 
 class GatedSaved:
     """What `gated_linear_backward` needs of a forward pass: x, w_gate and w_up (or copies that
-    the kernels read without another one) and the FP32 pre-activations (2, batch, out padded to
-    whole 16 bytes), and the problem: (element type, activation, batch, out, in, torch type,
-    device)."""
-    __slots__ = ("tensors", "problem")
+    the kernels read without another one; the caller's own must not be changed in between) and the
+    FP32 pre-activations (2, batch, out padded to whole 16 bytes), the problem (element type,
+    activation, batch, out, in, torch type, device), and where the three are padded copies in one
+    buffer, its size and their places."""
+    __slots__ = ("tensors", "problem", "places")
 
-    def __init__(self, tensors, problem):
-        self.tensors, self.problem = tensors, problem
+    def __init__(self, tensors, problem, places):
+        self.tensors, self.problem, self.places = tensors, problem, places
 
 
 # Up to _FEW_ROWS rows of 16-bit values run on the forward's few-rows kernel, which reads rows from
@@ -262,9 +267,10 @@ _FEW_ROWS, _FEW_VALUES = 4, 1 << 23
 
 
 def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int, few: bool = False):
-    """x and the weights as the kernels read them: three (buffer, element offset, leading
-    dimension, padded) and whether x and the weights are transposed.  Not padded: the buffer is
-    the tensor itself or a contiguous copy.  `few`: the few-rows kernel may take the operands."""
+    """x and the weights as the kernels read them, and their places: each one's element offset
+    and leading dimension, and whether x and the weights are transposed; then which of the
+    three are padded copies in one buffer, those being the buffer.  Not padded: the tensor itself
+    or a contiguous copy.  `few`: the few-rows kernel may take the operands."""
     (m, k), h = x.shape, w_gate.shape[0]
     if k == 1:
         # The imaginary part of a conjugate stands for its memory's negative.  Its elements are
@@ -297,13 +303,7 @@ def _operands(x, w_gate, w_up, per: int, aligned: bool, kind: int, index: int, f
             w_gate, og = buffer, offsets.pop(0)
         if pu:
             w_up, ou = buffer, offsets.pop(0)
-    return (x, ox, ldx, px), (w_gate, og, ldg, pg), (w_up, ou, ldu, pu), xt, gt
-
-
-def _matrix(operand, r: int, c: int, transposed: int) -> torch.Tensor:
-    """The (r, c) matrix that an operand of `_operands` holds."""
-    t, offset, ld, padded = operand
-    return t.as_strided((r, c), (1, ld) if transposed else (ld, 1), offset) if padded else t
+    return x, w_gate, w_up, (ox, ldx, og, ldg, ou, ldu, xt, gt), (px, pg, pu)
 
 
 def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: bool):
@@ -322,8 +322,8 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
     aligned = kind != sdk.FP32 or keep or m > 32
     few = kind != sdk.FP32 and not keep and (m == 1 or (m <= _FEW_ROWS and h * k <= _FEW_VALUES))
     with _on_device(index):
-        ops = _operands(x, w_gate, w_up, per, aligned, kind, index, few)
-        (xb, ox, ldx, _), (gb, og, ldg, _), (ub, ou, ldu, _), xt, wt = ops
+        x, w_gate, w_up, places, padded = _operands(x, w_gate, w_up, per, aligned, kind, index, few)
+        ox, ldx, og, ldg, ou, ldu, xt, wt = places
         out = x.new_empty((m, h))
         pre, pg0, pu0, ldp = None, 0, 0, 0
         if keep:
@@ -332,8 +332,8 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
             pg0 = pre.data_ptr()
             pu0 = pg0 + m * ldp * 4
         size = 16 // per
-        d = Gated(_GATED_SIZE, kind, act, xt, wt, 0, m, h, k, xb.data_ptr() + ox * size,
-                  gb.data_ptr() + og * size, ub.data_ptr() + ou * size, ldx, ldg, ldu,
+        d = Gated(_GATED_SIZE, kind, act, xt, wt, 0, m, h, k, x.data_ptr() + ox * size,
+                  w_gate.data_ptr() + og * size, w_up.data_ptr() + ou * size, ldx, ldg, ldu,
                   0 if bias_gate is None else bias_gate.data_ptr(),
                   0 if bias_up is None else bias_up.data_ptr(), pg0, pu0, ldp, 0, 0,
                   _stream(index))
@@ -343,8 +343,14 @@ def _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation: str, keep: b
             _check(st, "xvram_b200_gated_forward")
     if not keep:
         return out, None
-    saved = (_matrix(ops[0], m, k, xt), _matrix(ops[1], h, k, wt), _matrix(ops[2], h, k, wt), pre)
-    return out, GatedSaved(saved, (kind, act, m, h, k, dtype, device))
+    problem = (kind, act, m, h, k, dtype, device)
+    if all(padded):
+        return out, GatedSaved((x, pre), problem, (x.numel(), places))
+    saved = [t.as_strided((r, k), (1, ld) if tr else (ld, 1), o) if p else t
+             for t, r, o, ld, tr, p in ((x, m, ox, ldx, xt, padded[0]),
+                                        (w_gate, h, og, ldg, wt, padded[1]),
+                                        (w_up, h, ou, ldu, wt, padded[2]))]
+    return out, GatedSaved((*saved, pre), problem, None)
 
 
 def _gated_workspace(d, backward: int, like: torch.Tensor):
@@ -360,7 +366,8 @@ def _gated_workspace(d, backward: int, like: torch.Tensor):
 def gated_linear_forward(x, w_gate, w_up, bias_gate=None, bias_up=None, activation="silu"):
     """(h, saved): the gated block's result and what `gated_linear_backward` needs.  For callers
     that drive the backward pass themselves; autograd is not involved."""
-    _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
+    if _dual_level():
+        _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     with torch.no_grad():
         return _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
 
@@ -371,12 +378,15 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     `needs` does not ask for are None.  Sums are FP32; for float16 / bfloat16 the gradients of the
     pre-activations are rounded to the type once, as the tensor cores' operands (float16: times a
     power of two where its range would lose them, so that gradients which fit are right)."""
-    _refuse_tangents("gated_linear's backward", dh)
+    if _dual_level():
+        _refuse_tangents("gated_linear's backward", dh)
     kind, act, m, h, k, dtype, device = saved.problem
-    x, w_gate, w_up, pre = saved.tensors
+    *operands, pre = saved.tensors
+    places = saved.places
     # Strides are read from the tensors: autograd's saved-tensor hooks may have changed them.
     ldp = (h + 3) // 4 * 4
-    for t, shape, of in ((x, (m, k), dtype), (w_gate, (h, k), dtype), (w_up, (h, k), dtype),
+    shapes = ((m, k), (h, k), (h, k)) if places is None else ((places[0],),)
+    for t, shape, of in (*zip(operands, shapes, (dtype, dtype, dtype)),
                          (pre, (2, m, ldp), torch.float32)):
         if t.shape != shape or t.dtype != of or t.device != device:
             raise RuntimeError(f"a saved tensor of gated_linear must be {shape} {of} on {device} "
@@ -387,8 +397,14 @@ def gated_linear_backward(dh: torch.Tensor, saved: GatedSaved,
     with _on_device(index):
         if not pre.is_contiguous() or pre.data_ptr() % 16:
             pre = pre.clone(memory_format=torch.contiguous_format)
-        (x, ox, ldx, _), (w_gate, og, ldg, _), (w_up, ou, ldu, _), xt, wt = _operands(
-            x, w_gate, w_up, 16 // size, True, kind, index)
+        if places is None:
+            x, w_gate, w_up, place, _ = _operands(*operands, 16 // size, True, kind, index)
+        else:
+            x, place = operands[0], places[1]
+            if not x.is_contiguous() or x.data_ptr() % 16:
+                x = x.clone(memory_format=torch.contiguous_format)
+            w_gate = w_up = x
+        ox, ldx, og, ldg, ou, ldu, xt, wt = place
         dh, lddh = _rows(dh.detach() if dh.requires_grad else dh)
         dx = dh.new_empty((m, k)) if needs[0] else None
         dwg = dh.new_empty((h, k)) if needs[1] else None
@@ -411,14 +427,14 @@ class _GatedLinear(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, bias_gate, bias_up, activation):
         out, saved = _gated_forward(x, w_gate, w_up, bias_gate, bias_up, activation, True)
         ctx.save_for_backward(*saved.tensors)
-        ctx.problem = saved.problem
+        ctx.problem, ctx.places = saved.problem, saved.places
         return out
 
     @staticmethod
     def backward(ctx, dh):
         if torch.is_grad_enabled():  # create_graph=True
             raise RuntimeError("gated_linear has no second derivative")
-        saved = GatedSaved(ctx.saved_tensors, ctx.problem)
+        saved = GatedSaved(ctx.saved_tensors, ctx.problem, ctx.places)
         return (*gated_linear_backward(dh, saved, ctx.needs_input_grad), None)
 
 
@@ -432,7 +448,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     are read in place (16-bit ones where their base and leading dimension are multiples of 16
     bytes; others are copied first, unless there are up to four rows).  Differentiable once in every tensor argument, in reverse
     mode; tensors with a forward-mode tangent are refused."""
-    _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
+    if _dual_level():
+        _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     if torch.is_grad_enabled() and (
             x.requires_grad or w_gate.requires_grad or w_up.requires_grad or
             (bias_gate is not None and bias_gate.requires_grad) or
@@ -488,7 +505,8 @@ def quantize_mxfp4(x: torch.Tensor) -> Mxfp4Matrix:
         raise TypeError(f"quantize_mxfp4 takes float16, bfloat16 or float32 (got {x.dtype})")
     if x.dim() != 2:
         raise ValueError("expected a 2-D tensor")
-    _refuse_tangents("quantize_mxfp4", x)
+    if _dual_level():
+        _refuse_tangents("quantize_mxfp4", x)
     if x.device.type != "cuda":
         raise RuntimeError("quantize_mxfp4 needs a CUDA tensor (there is no CPU path)")
     if torch.is_grad_enabled() and x.requires_grad:
@@ -540,7 +558,8 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
     n = first.shape[0]
     if k == 0:
         raise ValueError(f"{what} needs at least one input feature")
-    _refuse_tangents(what, x, *biases)
+    if _dual_level():
+        _refuse_tangents(what, x, *biases)
     if device.type != "cuda" or first.codes.device != device or last.codes.device != device:
         raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
     if torch.is_grad_enabled() and (
