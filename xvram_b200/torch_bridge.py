@@ -469,13 +469,16 @@ class Mxfp4Matrix:
         rows, cols = shape
         if rows < 0 or cols < 0:
             raise ValueError("negative size")
-        for t, need, name in ((codes, rows * ((cols + 31) // 32) * 16, "codes"),
-                              (scales, ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
-                               "scales")):
-            if t.dtype != torch.uint8 or t.numel() != need or not t.is_contiguous() or \
-                    t.data_ptr() % 16:
-                raise ValueError(f"{name} of a ({rows}, {cols}) MXFP4 matrix must be {need} "
-                                 "contiguous bytes (uint8), 16-byte aligned")
+        need = rows * ((cols + 31) // 32) * 16
+        if codes.dtype is not torch.uint8 or codes.numel() != need or \
+                not codes.is_contiguous() or codes.data_ptr() % 16:
+            raise ValueError(f"codes of a ({rows}, {cols}) MXFP4 matrix must be {need} "
+                             "contiguous bytes (uint8), 16-byte aligned")
+        need = ((rows + 127) // 128) * ((cols + 127) // 128) * 512
+        if scales.dtype is not torch.uint8 or scales.numel() != need or \
+                not scales.is_contiguous() or scales.data_ptr() % 16:
+            raise ValueError(f"scales of a ({rows}, {cols}) MXFP4 matrix must be {need} "
+                             "contiguous bytes (uint8), 16-byte aligned")
         if codes.device != scales.device:
             raise ValueError("codes and scales must be on the same device")
         self.codes, self.scales, self.shape = codes, scales, (rows, cols)
@@ -542,15 +545,16 @@ def dequantize_mxfp4(q: Mxfp4Matrix, dtype: torch.dtype = torch.float32) -> torc
     return out
 
 
-def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) -> torch.Tensor:
-    """The product `call` of x and one or two MXFP4 weights, its arguments checked."""
+def _mxfp4_product(x, first, last, bias0, bias1, activation: int, dtype, what: str,
+                   call) -> torch.Tensor:
+    """The product `call` of x and one (first is last) or two MXFP4 weights, its arguments
+    checked."""
     quantised = isinstance(x, Mxfp4Matrix)
     given = torch.float32 if quantised else x.dtype
     dtype = given if dtype is None else dtype
     if dtype not in _FEED_TYPES or given not in _FEED_TYPES:
         raise TypeError(f"{what} supports float16, bfloat16 and float32 (got {given} to {dtype})")
     shape, device = x.shape, x.device
-    first, last = weights[0], weights[-1]
     if not isinstance(first, Mxfp4Matrix) or not isinstance(last, Mxfp4Matrix) or \
             len(shape) != 2 or first.shape[1] != shape[1] or last.shape != first.shape:
         raise ValueError(f"{what} takes x (batch, in) and MXFP4 weights (out, in)")
@@ -559,12 +563,13 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
     if k == 0:
         raise ValueError(f"{what} needs at least one input feature")
     if _dual_level():
-        _refuse_tangents(what, x, *biases)
+        _refuse_tangents(what, x, bias0, bias1)
     if device.type != "cuda" or first.codes.device != device or last.codes.device != device:
         raise RuntimeError(f"{what} needs its operands on one CUDA device (there is no CPU path)")
     if torch.is_grad_enabled() and (
             (not quantised and x.requires_grad) or
-            any(b is not None and b.requires_grad for b in biases)):
+            (bias0 is not None and bias0.requires_grad) or
+            (bias1 is not None and bias1.requires_grad)):
         raise RuntimeError(f"{what} has no gradient: detach its input and biases")
     index = device.index
     with _on_device(index):
@@ -580,12 +585,20 @@ def _mxfp4_product(x, weights, biases, activation: int, dtype, what: str, call) 
             codes = buffer.data_ptr()
             scales = codes + size
         out = like.new_empty((m, n), dtype=dtype)
-        b = [None if t is None else _check_bias(t, n, dtype, device, "bias") for t in biases]
+        b0 = b1 = 0
+        if bias0 is not None:
+            bias0 = _check_bias(bias0, n, dtype, device, "bias")
+            b0 = bias0.data_ptr()
+        if bias1 is not None:
+            bias1 = _check_bias(bias1, n, dtype, device, "bias")
+            b1 = bias1.data_ptr()
         d = Mxfp4Product(_PRODUCT_SIZE, _FEED_TYPES[given], _FEED_TYPES[dtype], activation, m, n, k,
                          src, ldx, codes, scales, first.codes.data_ptr(), last.codes.data_ptr(),
-                         first.scales.data_ptr(), last.scales.data_ptr(), _ptr(b[0]), _ptr(b[-1]),
+                         first.scales.data_ptr(), last.scales.data_ptr(), b0, b1,
                          out.data_ptr(), n, _stream(index))
-        _check(call(ctypes.byref(d)), what)
+        st = call(ctypes.byref(d))
+        if st:
+            _check(st, what)
     return out
 
 
@@ -595,7 +608,7 @@ def linear_mxfp4(x, weight: Mxfp4Matrix, bias: torch.Tensor | None = None, relu:
     operands, FP32 accumulation, rounded once.  x: (batch, in), a float tensor that is quantised
     here or an Mxfp4Matrix; weight: (out, in).  The result (and the bias) has `dtype`: x's type by
     default, float32 for an Mxfp4Matrix.  Inference only: no gradient."""
-    return _mxfp4_product(x, (weight,), (bias,), 1 if relu else 0, dtype, "linear_mxfp4",
+    return _mxfp4_product(x, weight, weight, bias, None, 1 if relu else 0, dtype, "linear_mxfp4",
                           lib.xvram_b200_mxfp4_linear)
 
 
@@ -604,7 +617,7 @@ def gated_linear_mxfp4(x, w_gate: Mxfp4Matrix, w_up: Mxfp4Matrix,
                        activation: str = "silu", dtype: torch.dtype | None = None) -> torch.Tensor:
     """`gated_linear` over MXFP4 operands, with `linear_mxfp4`'s input and types: both products,
     the biases, the activation and the product of the two in one kernel.  No gradient."""
-    return _mxfp4_product(x, (w_gate, w_up), (bias_gate, bias_up), _activation(activation), dtype,
+    return _mxfp4_product(x, w_gate, w_up, bias_gate, bias_up, _activation(activation), dtype,
                           "gated_linear_mxfp4", lib.xvram_b200_mxfp4_gated)
 
 
