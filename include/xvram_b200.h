@@ -444,7 +444,8 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_forward(const xvram_b200
  * it is not wanted.  Gradients have the data type and are stored with contiguous rows whatever
  * the operands' transposition.  For FP16 / BF16 the gradients of the pre-activations are rounded
  * to the data type once, as the tensor cores' operands (FP16: times a power of two, where its range
- * would lose them); all sums are FP32.  Results do not depend on timing.  With m = 0 the weights' and biases' gradients are zeros. */
+ * would lose them); all sums are FP32.  Results do not depend on timing.  With m = 0 the weights'
+ * and biases' gradients are zeros. */
 XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_gated_backward(
     const xvram_b200_gated_v1* problem, uint64_t dout, int64_t ld_dout, uint64_t dx, int64_t ld_dx,
     uint64_t dw_gate, uint64_t dw_up, int64_t ld_dw, uint64_t db_gate, uint64_t db_up);
@@ -481,9 +482,9 @@ XVRAM_B200_API xvram_status XVRAM_CALL xvram_b200_mxfp4_dequantize(
  * once the call's work on `stream` is done); up to XVRAM_B200_MXFP4_DIRECT_ROWS rows of at most
  * XVRAM_B200_MXFP4_DIRECT_VALUES values together can be quantised inside the product instead:
  * with x_codes and x_scales 0 they are, and with that memory given where it is faster (from
- * about half of these values on it seldom is).  With x = 0, x_codes and x_scales as they are.  Biases (0 for
- * none) hold n values of out_type.  XVRAM_STATUS_UNSUPPORTED: quantised inside the product, a row this
- * long needs larger clusters than the device runs; quantise it first.
+ * about half of these values on it seldom is).  With x = 0, x_codes and x_scales as they are.
+ * Biases (0 for none) hold n values of out_type.  XVRAM_STATUS_UNSUPPORTED: quantised inside the
+ * product, a row this long needs larger clusters than the device runs; quantise it first.
  */
 #define XVRAM_B200_MXFP4_DIRECT_ROWS 16
 #define XVRAM_B200_MXFP4_DIRECT_VALUES 65536

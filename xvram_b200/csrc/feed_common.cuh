@@ -55,7 +55,7 @@ struct Params {
   int tiles_m, tiles_n, batches;
   int a_mn, b_mn;         // 16-bit operands stored M-/N-major
   int act, relu;
-  const unsigned* top;    // FP16, plain: the A operands hold their values times fp16_scale(*top); 0: once
+  const unsigned* top;    // FP16, plain: A holds its values times fp16_scale(*top); null: as they are
   int unit;               // widest access the output rows allow, in bytes (store_unit)
   uint32_t idesc;
   const void *bias0, *bias1;
@@ -183,7 +183,8 @@ __device__ __forceinline__ void logistic(float v, float& q, float& complement) {
   complement = v < 0.0f ? r : er;
 }
 // q alone.  FAST, in the tensor cores' epilogues: the direct form, two instructions shorter (MXFP4
-// 4096 x 512 x 8192 57 us against 80).  1 + exp(-v) from 2^126 on gives zero, which is off by q < 2^-126.
+// 4096 x 512 x 8192 57 us against 80).  1 + exp(-v) from 2^126 on gives zero, which is off by
+// q < 2^-126.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float v) {
   if constexpr (FAST)

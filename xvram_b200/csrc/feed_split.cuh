@@ -1,5 +1,6 @@
 // feed_split.cuh -- the tensor-core kernel of the feed-forward operators for at most 128 rows, and
-// for more where CTA pairs would find too few tiles (operands, epilogues and the accumulator's columns: feed_common.cuh).
+// for more where CTA pairs would find too few tiles (operands, epilogues and the accumulator's
+// columns: feed_common.cuh).
 //
 // Bound by reading the weights from HBM: a 128 x 256 accumulator takes all rows of A, so each
 // weight is read once, and M = 128 MMAs on fewer rows still finish inside the time of the

@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(256)
   }
   if (kRange && !again && top) {
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0 && most > *static_cast<volatile unsigned*>(top)) // a maximum: any order, the same bits
-      atomicMax(top, most);
+    if (lane == 0 && most > *static_cast<volatile unsigned*>(top))
+      atomicMax(top, most); // the same bits in any order
   }
   if (!partial)
     return;
@@ -464,12 +464,12 @@ cudaError_t forward_rows(const GatedProblem& q, void* out, long long ldo, cudaSt
 // Whether the forward runs on the few-rows kernel.  It reads each weight once per 8 rows of x and
 // sustains about 20 TFLOP/s of FP32 FMAs; measured against the tile kernels (device time,
 // weights larger than L2 rotated):
-//   FP32, 4096 inputs, 8192 features: 46 us for 2 rows (5.8 TB/s), 431 for 64, 865 for 128, against
-//   548 us for the FFMA kernel, whose waves of 148 128 x 128 tiles take 0.066 us per input whatever
+//   FP32, 4096 inputs, 8192 features: 44 us for 2 rows (6.1 TB/s), 399 for 64, 865 for 128, against
+//   549 us for the FFMA kernel, whose waves of 148 128 x 128 tiles take 0.066 us per input whatever
 //   m is; 1024 x 2048: 62 us for 128 rows against 136.  4 m h k / 20 TFLOP/s is below the two GEMMs'
 //   2 x 0.066 us k waves while m h < 640k waves.
-//   BF16: 4096 x 8192 25 us for one row, 34 for 4, against the tensor cores' 26; 1024 x 2048 4.2 us for
-//   one row and 4.9 for 4, against 7.
+//   BF16: 4096 x 8192 22.6 us for one row, 34 for 4, against the tensor cores' 25.7; 1024 x 2048 3.4 us
+//   for one row and 4.5 for 4, against 7.
 bool few_rows(const GatedProblem& q) {
   if (q.x_transposed || q.w_transposed)
     return false;

@@ -446,8 +446,9 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
     gelu, gelu_tanh, relu or sigmoid.  float16 / bfloat16 run as one tensor-core kernel with FP32
     accumulation and one rounding, float32 in strict FP32.  Row-major and transposed operands
     are read in place (16-bit ones where their base and leading dimension are multiples of 16
-    bytes; others are copied first, unless there are up to four rows).  Differentiable once in every tensor argument, in reverse
-    mode; tensors with a forward-mode tangent are refused."""
+    bytes; others are copied first, unless the call runs on the few-rows kernel: one row, or up to
+    four with weights of up to 2^23 values).  Differentiable once in every tensor argument, in
+    reverse mode; tensors with a forward-mode tangent are refused."""
     if _dual_level():
         _refuse_tangents("gated_linear", x, w_gate, w_up, bias_gate, bias_up)
     if torch.is_grad_enabled() and (
